@@ -19,8 +19,8 @@
  * aborts: every entry point returns a kcg_status.
  *
  * All entry points are thread-safe and hold no state between calls.  A call may
- * issue more than one kernel on the stream.  No tensor may have 2^31 elements
- * or more (KCG_ERR_UNSUPPORTED_SHAPE): the one run with a larger operand ended in a GPU
+ * issue more than one kernel on the stream.  No tensor but a key/value cache may have 2^31
+ * elements or more (KCG_ERR_UNSUPPORTED_SHAPE): the one run with a larger operand ended in a GPU
  * memory fault whose cause is not known (a host replay of the matmul kernel's address
  * arithmetic, tests/gemm_dl_address_model.cc, finds every access of that call inside its
  * tensor).  The largest operand that has been run on the GPU is 1 GiB; operands between
@@ -206,7 +206,9 @@ KCG_API int kcg_fmha_f32(const float *Q, const float *K, const float *V, float *
                          int32_t B, int32_t H, int32_t S, int32_t D, float scale,
                          int causal, const kcg_fmha_sched *sched, void *stream);
 
-typedef enum kcg_dtype { KCG_F32 = 0, KCG_BF16 = 1 } kcg_dtype;
+/* KCG_E4M3 (8 bits: sign, 4 exponent bits of bias 7, 3 mantissa bits, no infinity, NaN 0x7f) is
+ * a type of key/value caches only. */
+typedef enum kcg_dtype { KCG_F32 = 0, KCG_BF16 = 1, KCG_E4M3 = 2 } kcg_dtype;
 
 /* Same, with Q, K, V holding bf16 bit patterns (extension: the reference knows
  * only float32/float64/float16, src/Frontend/Operators.cc:5-10).  Products are
@@ -251,6 +253,112 @@ KCG_API int kcg_batched_matmul_f32(const float *A, int transA, const float *B,
  * the reference's literal form is finite, and stays finite where that form overflows
  * (x > 88 gives inf / inf = NaN there).  A deliberate deviation. */
 KCG_API int kcg_softmax_f32(float *x, int64_t rows, int64_t n, void *stream);
+
+/* ---- attention layers that serve: heads before, and keys and values in, a paged cache ----- */
+
+/* Everything in this section is an extension: the reference has no normalisation, no position
+ * rotation and no cache.  The entry points form one chain: kcg_qk_norm_rope makes the queries
+ * and keys that kcg_fmha_* and the cache take, kcg_kv_cache_write puts new keys and values into
+ * the cache, kcg_fmha_cache attends over it, kcg_kv_cache_read brings cached tokens back as
+ * rows (a prefill that continues a cached prefix runs kcg_fmha_* on them).
+ *
+ * kcg_rows: a tensor [B][S][H][D] whose rows of D elements are contiguous.  Strides are in
+ * elements, 0 or more; a tensor that is written has rows that do not overlap (else
+ * KCG_ERR_BAD_ARGUMENT).  Rows that all start on 16-byte boundaries are read and written 16 bytes
+ * at a time, any other element-aligned rows one element at a time.  [B][H][S][D] memory, a part of
+ * a fused projection's output and [tokens][H][D] (B = 1) are all such tensors.  No tensor of
+ * this kind may have 2^31 elements or more; a cache may (its addresses are 64 bits wide). */
+typedef struct kcg_rows {
+  void *data;
+  int64_t stride_b, stride_s, stride_h;
+} kcg_rows;
+
+/* Per-head RMS norm and position rotation of queries and keys in one pass:
+ *   y = weight * x * (mean(x^2) + eps)^(-1/2)   over the D elements of a head, then each of the
+ *   rot_dim / 2 pairs (a, b) of y becomes (a cos t - b sin t, b cos t + a sin t),
+ *   t = positions[b][s] * inv_freq[pair];
+ * interleaved = 0 pairs elements i and i + rot_dim / 2, 1 pairs 2i and 2i + 1; elements from
+ * rot_dim on are not rotated.  q is [B][S][Hq][D], k [B][S][Hk][D], positions [B][S] and
+ * inv_freq [rot_dim / 2] contiguous; everything but inv_freq (fp32) and positions (int32) is of
+ * `dtype` (KCG_F32 or KCG_BF16).  Arithmetic is fp32 (angles: 64 bits), one rounding at the end.
+ * D is 64 or 128; rot_dim a multiple of 16 from 16 to D.  An output may be its own input (same
+ * data and strides); otherwise outputs overlap no input. */
+KCG_API int kcg_qk_norm_rope(const kcg_rows *q, const kcg_rows *k, const kcg_rows *q_out,
+                             const kcg_rows *k_out, const void *q_weight, const void *k_weight,
+                             const int32_t *positions, const float *inv_freq, int dtype, int32_t B,
+                             int32_t S, int32_t Hq, int32_t Hk, int32_t D, int32_t rot_dim,
+                             int interleaved, float eps, void *stream);
+
+/* Its gradient: from dq, dk (of the outputs) and the inputs of the forward call, grad_q and grad_k
+ * (of the inputs) and the weights' gradients [D], all of `dtype`.  The sums over tokens and heads
+ * are fp32 and taken in a fixed order: results do not vary between runs.  `workspace`: 16-byte
+ * aligned device memory of at least kcg_qk_norm_rope_backward_ws_bytes(...) bytes that nothing
+ * else uses until the call has completed (fewer bytes: KCG_ERR_BAD_ARGUMENT).  grad_q may be dq,
+ * grad_k may be dk. */
+KCG_API int64_t kcg_qk_norm_rope_backward_ws_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hk,
+                                                   int32_t D);
+KCG_API int kcg_qk_norm_rope_backward(const kcg_rows *dq, const kcg_rows *dk, const kcg_rows *q,
+                                      const kcg_rows *k, const kcg_rows *grad_q,
+                                      const kcg_rows *grad_k, const void *q_weight,
+                                      const void *k_weight, void *grad_q_weight,
+                                      void *grad_k_weight, const int32_t *positions,
+                                      const float *inv_freq, int dtype, int32_t B, int32_t S,
+                                      int32_t Hq, int32_t Hk, int32_t D, int32_t rot_dim,
+                                      int interleaved, float eps, void *workspace,
+                                      int64_t workspace_bytes, void *stream);
+
+/* A paged key/value cache: k and v are [pages][heads][page_size][dim] of KCG_BF16 or KCG_E4M3.
+ * An e4m3 row stands for its values times 2^(x - 127), x its byte in k_exp / v_exp
+ * [pages][heads][page_size] (NULL for bf16).  A power of two keeps every dequantised value a
+ * bf16 number.  page_size is 16, 32, 64, 128 or 256, dim 64 or 128; all pointers 16-byte
+ * aligned.  A token's slot is page * page_size + its place in the page. */
+typedef struct kcg_kv_cache {
+  void *k, *v;
+  uint8_t *k_exp, *v_exp;
+  int32_t dtype, pages, page_size, heads, dim;
+} kcg_kv_cache;
+
+/* Writes keys and values [B][S][heads][dim] of `dtype` (KCG_F32 or KCG_BF16) to the slots
+ * slots[B][S].  e4m3: x is the least exponent (at least 1) with which the largest finite magnitude
+ * of the row does not exceed 448; values are rounded to nearest, halves to even; infinities and
+ * NaN are stored as NaN.  A token whose slot lies outside the cache (-1: padding) is not written;
+ * of tokens with the same slot the last one is.  Slots that no token names stay as they were. */
+KCG_API int kcg_kv_cache_write(const kcg_kv_cache *cache, const kcg_rows *k, const kcg_rows *v,
+                               int dtype, const int32_t *slots, int32_t B, int32_t S,
+                               void *stream);
+
+/* The reverse: keys and values of the slots as rows of `dtype`.  A slot outside the cache gives
+ * rows of zeros. */
+KCG_API int kcg_kv_cache_read(const kcg_kv_cache *cache, const int32_t *slots, const kcg_rows *k,
+                              const kcg_rows *v, int dtype, int32_t B, int32_t S, void *stream);
+
+/* Attention of the newest N tokens of each of B sequences over the cache: one token, a chain of
+ * drafted tokens or a tree of them.  Sequence b holds keys 0 .. context_lens[b] - 1 and, behind
+ * them, the keys of its draft_lens[b] drafted tokens (NULL: N each), all already written; key j is in
+ * page block_table[b][j / page_size] (block_table [B][table_width]).  The query of drafted token n sees
+ * the whole context, and of the drafted keys those whose bit is set in tree_mask[b][n] (bit 0: the
+ * first one).  NULL: a chain, bits 0 .. n.  O = softmax(scale * q.K^T) . V over the keys that are
+ * seen; a query that sees none gets zeros.  Keys and values that a query does not see have no
+ * influence on it, whatever they hold.
+ *
+ * q is bf16 [B][N][Hq][dim]; out [B][N][Hq][dim] of o_dtype (KCG_BF16 or KCG_F32); Hq a multiple of
+ * the cache's heads, query head h reading head h / (Hq / heads); N from 1 to 64.  Rows of `out` from
+ * draft_lens[b] on stay as they were.  Products are bf16 x bf16 in fp32, the softmax fp32; the
+ * weights are rounded to bf16 for the second product (fp32 output: split over three bf16 numbers).
+ * Lengths below 0 count as 0, draft_lens above N as N; keys beyond the table's last page and keys in
+ * pages outside the cache are not seen.
+ *
+ * `workspace`: 16-byte aligned device memory that nothing else uses until the call has
+ * completed, for partial results where the keys of a sequence are split over several workgroups.
+ * kcg_fmha_cache_ws_bytes gives the bytes the preferred split needs (0: none); with fewer, or NULL,
+ * the call splits less, down to not at all. */
+KCG_API int64_t kcg_fmha_cache_ws_bytes(const kcg_kv_cache *cache, int32_t table_width, int32_t B,
+                                        int32_t N, int32_t Hq);
+KCG_API int kcg_fmha_cache(const kcg_rows *q, const kcg_kv_cache *cache, const int32_t *block_table,
+                           int32_t table_width, const int32_t *context_lens,
+                           const int32_t *draft_lens, const uint64_t *tree_mask,
+                           const kcg_rows *out, int o_dtype, int32_t B, int32_t N, int32_t Hq,
+                           float scale, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

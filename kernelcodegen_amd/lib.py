@@ -36,6 +36,17 @@ class FmhaSched(ctypes.Structure):
     _fields_ = [("br", _i32), ("bc", _i32)]
 
 
+class Rows(ctypes.Structure):
+    """kcg_rows: a [B,S,H,D] tensor with contiguous rows of D elements; strides in elements."""
+    _fields_ = [("data", _vp), ("stride_b", _i64), ("stride_s", _i64), ("stride_h", _i64)]
+
+
+class KvCache(ctypes.Structure):
+    """kcg_kv_cache: a paged key/value cache."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_exp", _vp), ("v_exp", _vp), ("dtype", _i32), ("pages", _i32),
+                ("page_size", _i32), ("heads", _i32), ("dim", _i32)]
+
+
 class LaunchInfo(ctypes.Structure):
     _fields_ = [("grid", _i32 * 3), ("block", _i32 * 3), ("lds_bytes", _i32),
                 ("waves_per_block", _i32), ("kernel", ctypes.c_char * 64),
@@ -43,6 +54,9 @@ class LaunchInfo(ctypes.Structure):
                 ("tail_grid", _i32 * 3), ("tail_block", _i32 * 3), ("tail_lds_bytes", _i32),
                 ("tail_kernel", ctypes.c_char * 64)]
 
+
+_rows = ctypes.POINTER(Rows)
+_cache = ctypes.POINTER(KvCache)
 
 # name -> (restype, argtypes); every symbol include/kcg.h declares.
 SYMBOLS = {
@@ -69,6 +83,16 @@ SYMBOLS = {
     "kcg_batched_matmul_f32": (ctypes.c_int, [_vp, ctypes.c_int, _vp, ctypes.c_int, _vp, _i64,
                                               _i64, _i64, _i64, _vp]),
     "kcg_softmax_f32": (ctypes.c_int, [_vp, _i64, _i64, _vp]),
+    "kcg_qk_norm_rope": (ctypes.c_int, [_rows] * 4 + [_vp] * 4 + [ctypes.c_int] + [_i32] * 6
+                         + [ctypes.c_int, ctypes.c_float, _vp]),
+    "kcg_qk_norm_rope_backward_ws_bytes": (_i64, [_i32] * 5),
+    "kcg_qk_norm_rope_backward": (ctypes.c_int, [_rows] * 6 + [_vp] * 6 + [ctypes.c_int] + [_i32] * 6
+                                  + [ctypes.c_int, ctypes.c_float, _vp, _i64, _vp]),
+    "kcg_kv_cache_write": (ctypes.c_int, [_cache, _rows, _rows, ctypes.c_int, _vp, _i32, _i32, _vp]),
+    "kcg_kv_cache_read": (ctypes.c_int, [_cache, _vp, _rows, _rows, ctypes.c_int, _i32, _i32, _vp]),
+    "kcg_fmha_cache_ws_bytes": (_i64, [_cache, _i32, _i32, _i32, _i32]),
+    "kcg_fmha_cache": (ctypes.c_int, [_rows, _cache, _vp, _i32, _vp, _vp, _vp, _rows, ctypes.c_int, _i32, _i32, _i32,
+                                      ctypes.c_float, _vp, _i64, _vp]),
 }
 
 

@@ -5,6 +5,10 @@ Names and argument meaning follow the reference's Frontend operators
 and the fused attention the FMHAOptimizer recognises
 (src/Optimizer/Optimizer.cc:586-672).  Everything goes through the C-ABI; a
 failing status raises lib.KcgError.
+
+Attention layers that serve have operators of their own (the reference has none):
+qk_norm_rope and its gradient make the queries and keys, KvCache with kv_cache_write and
+kv_cache_read holds them, fmha_cache attends over it.
 """
 import ctypes
 
@@ -16,6 +20,8 @@ EPILOGUE_NONE = 0
 EPILOGUE_RELU = 1
 F32 = 0
 BF16 = 1
+E4M3 = 2
+_DTYPES = {torch.float32: F32, torch.bfloat16: BF16}
 
 
 def _ptr(t):
@@ -173,4 +179,253 @@ def fmha(Q, K, V, scale=1.0, causal=False, out=None, out_dtype=None, sched=None)
                              float(scale), int(causal), _sched(sched, lib.FmhaSched),
                              lib.current_stream())
     lib.check(st)
+    return out
+
+
+# ---- attention layers that serve --------------------------------------------------------
+
+
+def _rows(t, name, dtype, device, shape=None):
+    """A [B,S,H,D] (or [tokens,H,D]) tensor with any strides but a contiguous last axis."""
+    if not isinstance(t, torch.Tensor) or t.dim() not in (3, 4):
+        raise ValueError("%s must be a [B,S,H,D] or [tokens,H,D] tensor" % name)
+    if not t.is_cuda or t.device != device:
+        raise ValueError("%s must be on device %s" % (name, device))
+    if t.dtype != dtype:
+        raise ValueError("%s must have dtype %s, not %s" % (name, dtype, t.dtype))
+    if shape is not None and t.shape != shape:
+        raise ValueError("%s must have shape %s, not %s" % (name, tuple(shape), tuple(t.shape)))
+    stride = t.stride()
+    if stride[-1] != 1:
+        raise ValueError("the last axis of %s must be contiguous" % name)
+    return lib.Rows(t.data_ptr(), stride[0] if len(stride) == 4 else 0, stride[-3], stride[-2])
+
+
+def _call(fn, device, *args):
+    """Calls a C entry point on the current stream of `device`, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        st = fn(*args, lib.current_stream())
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, lib.current_stream())
+    if st:
+        lib.check(st)
+
+
+def _workspace(workspace, need, device, name="workspace"):
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    if not (isinstance(workspace, torch.Tensor) and workspace.is_cuda and workspace.device == device
+            and workspace.is_contiguous()):
+        raise ValueError("%s must be a contiguous tensor on %s" % (name, device))
+    return workspace
+
+
+def _bytes(t):
+    return t.numel() * t.element_size()
+
+
+def _norm_rope_args(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved):
+    if not isinstance(q, torch.Tensor) or q.dtype not in _DTYPES or not q.is_cuda or q.dim() not in (3, 4):
+        raise ValueError("q must be a float32 or bfloat16 device tensor [B,S,H,D] or [tokens,H,D]")
+    device, dtype = q.device, q.dtype
+    rq, rk = _rows(q, "q", dtype, device), _rows(k, "k", dtype, device)
+    if k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+        raise ValueError("k must have q's tokens and head dimension")
+    D = q.shape[-1]
+    _check(q_weight, "q_weight", dtype, (D,), device)
+    _check(k_weight, "k_weight", dtype, (D,), device)
+    _check(positions, "positions", torch.int32, q.shape[:-2], device)
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1:
+        raise ValueError("inv_freq must be a tensor of one frequency for each rotated pair")
+    _check(inv_freq, "inv_freq", torch.float32, inv_freq.shape, device)
+    B = q.shape[0] if q.dim() == 4 else 1
+    tail = (positions.data_ptr(), inv_freq.data_ptr(), _DTYPES[dtype], B, q.shape[-3], q.shape[-2], k.shape[-2], D,
+            2 * inv_freq.shape[0], int(bool(interleaved)), eps)
+    return rq, rk, tail
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False, out=None):
+    """Per-head RMS norm with a learned weight, then the position rotation, of q and k in one pass.
+
+    q [B,S,Hq,D] and k [B,S,Hk,D] (or [tokens,H,D]) may have any strides but a contiguous
+    last axis, so parts of a fused projection's output are taken as they are.  positions: int32
+    [B,S]; inv_freq: fp32, one frequency per rotated pair (2 * len(inv_freq) elements of a head
+    are rotated: elements i and i + len, or 2i and 2i + 1 if `interleaved`).  Returns the new
+    (q, k), written to the pair `out` if given; out=(q, k) works in place.  kcg_qk_norm_rope.
+    """
+    rq, rk, tail = _norm_rope_args(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    if out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    else:
+        q_out, k_out = out
+    ro = _rows(q_out, "out[0]", q.dtype, q.device, q.shape)
+    rp = _rows(k_out, "out[1]", q.dtype, q.device, k.shape)
+    _call(lib.load().kcg_qk_norm_rope, q.device, rq, rk, ro, rp, q_weight.data_ptr(), k_weight.data_ptr(), *tail)
+    return q_out, k_out
+
+
+def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False,
+                          workspace=None):
+    """Gradients (q, k, q_weight, k_weight) of qk_norm_rope from those of its outputs.
+
+    The other arguments are the forward call's inputs.  workspace: a contiguous device tensor
+    of at least kcg_qk_norm_rope_backward_ws_bytes bytes (allocated if not given).
+    """
+    rq, rk, tail = _norm_rope_args(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    rdq = _rows(dq, "dq", q.dtype, q.device, q.shape)
+    rdk = _rows(dk, "dk", q.dtype, q.device, k.shape)
+    L = lib.load()
+    gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    gk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    gwq, gwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
+    rgq, rgk = _rows(gq, "grad_q", q.dtype, q.device), _rows(gk, "grad_k", q.dtype, q.device)
+    ws = _workspace(workspace, L.kcg_qk_norm_rope_backward_ws_bytes(*tail[3:8]), q.device)
+    if ws is None:  # a shape that the call itself refuses
+        ws = torch.empty(16, dtype=torch.uint8, device=q.device)
+    _call(L.kcg_qk_norm_rope_backward, q.device, rdq, rdk, rq, rk, rgq, rgk, q_weight.data_ptr(), k_weight.data_ptr(),
+          gwq.data_ptr(), gwk.data_ptr(), *tail, ws.data_ptr(), _bytes(ws))
+    return gq, gk, gwq, gwk
+
+
+class KvCache:
+    """A paged key/value cache over tensors of the caller.
+
+    k, v: [pages, heads, page_size, dim], bfloat16 or float8_e4m3fn, contiguous; for
+    float8_e4m3fn also k_exp, v_exp: uint8 [pages, heads, page_size], a row standing for its
+    values times 2^(exponent - 127).  page_size is 16, 32, 64, 128 or 256, dim 64 or 128.  The
+    handle keeps the tensors alive and their addresses at hand: they must not be resized.
+    """
+
+    def __init__(self, k, v, k_exp=None, v_exp=None):
+        if not isinstance(k, torch.Tensor) or k.dim() != 4 or not k.is_cuda:
+            raise ValueError("k must be a [pages, heads, page_size, dim] device tensor")
+        if k.dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError("a cache holds bfloat16 or float8_e4m3fn, not %s" % k.dtype)
+        _check(k, "k", k.dtype, k.shape, k.device)
+        _check(v, "v", k.dtype, k.shape, k.device)
+        if k.dtype == torch.float8_e4m3fn:
+            _check(k_exp, "k_exp", torch.uint8, k.shape[:3], k.device)
+            _check(v_exp, "v_exp", torch.uint8, k.shape[:3], k.device)
+        elif k_exp is not None or v_exp is not None:
+            raise ValueError("a bfloat16 cache has no exponents")
+        self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
+        self.device = k.device
+        pages, self.heads, self.page_size, self.dim = k.shape
+        eight = k.dtype == torch.float8_e4m3fn
+        if max(k.shape) > 0x7fffffff:
+            raise ValueError("the cache's extents must be 32-bit numbers")
+        self._c = lib.KvCache(k.data_ptr(), v.data_ptr(), k_exp.data_ptr() if eight else None,
+                              v_exp.data_ptr() if eight else None, E4M3 if eight else BF16, pages, self.page_size,
+                              self.heads, self.dim)
+
+    @classmethod
+    def empty(cls, pages, heads, page_size, dim, dtype=torch.float8_e4m3fn, device="cuda"):
+        """A cache with memory of its own.  What it holds before the first write is undefined."""
+        k, v = (torch.empty((pages, heads, page_size, dim), dtype=dtype, device=device) for _ in range(2))
+        if dtype != torch.float8_e4m3fn:
+            return cls(k, v)
+        return cls(k, v, *(torch.empty((pages, heads, page_size), dtype=torch.uint8, device=device) for _ in range(2)))
+
+
+def _cache_check(cache):
+    if not isinstance(cache, KvCache):
+        raise ValueError("cache must be a KvCache")
+    return cache.device
+
+
+def kv_cache_write(cache, k, v, slots):
+    """Writes keys and values [B,S,heads,dim] (or [tokens,heads,dim]) to the int32 slots [B,S].
+
+    A slot is page * page_size + place; -1 (padding) and any other slot outside the cache is
+    not written, and of tokens with the same slot the last one is.  fp32 or bf16 rows are
+    rounded to the cache's type; kcg_kv_cache_write says how.
+    """
+    device = _cache_check(cache)
+    if not isinstance(k, torch.Tensor) or k.dtype not in _DTYPES:
+        raise ValueError("k must be a float32 or bfloat16 tensor")
+    rk = _rows(k, "k", k.dtype, device)
+    rv = _rows(v, "v", k.dtype, device, k.shape)
+    if k.shape[-2:] != (cache.heads, cache.dim):
+        raise ValueError("k must have the cache's heads and dim %s" % ((cache.heads, cache.dim),))
+    _check(slots, "slots", torch.int32, k.shape[:-2], device)
+    B = k.shape[0] if k.dim() == 4 else 1
+    _call(lib.load().kcg_kv_cache_write, device, cache._c, rk, rv, _DTYPES[k.dtype], slots.data_ptr(), B, k.shape[-3])
+
+
+def kv_cache_read(cache, slots, out_dtype=torch.bfloat16, out=None):
+    """Keys and values of the int32 slots [B,S] (or [tokens]) as rows [..., heads, dim].
+
+    A slot outside the cache gives rows of zeros.  out: the pair of tensors to write, with any
+    strides but a contiguous last axis.
+    """
+    device = _cache_check(cache)
+    if not isinstance(slots, torch.Tensor) or slots.dim() not in (1, 2):
+        raise ValueError("slots must be an int32 tensor [B,S] or [tokens]")
+    _check(slots, "slots", torch.int32, slots.shape, device)
+    shape = torch.Size(tuple(slots.shape) + (cache.heads, cache.dim))
+    if out is None:
+        k = torch.empty(shape, dtype=out_dtype, device=device)
+        v = torch.empty(shape, dtype=out_dtype, device=device)
+    else:
+        k, v = out
+    dtype = k.dtype if isinstance(k, torch.Tensor) else None
+    if dtype not in _DTYPES:
+        raise ValueError("a cache is read as float32 or bfloat16")
+    rk, rv = _rows(k, "out[0]", dtype, device, shape), _rows(v, "out[1]", dtype, device, shape)
+    B = slots.shape[0] if slots.dim() == 2 else 1
+    _call(lib.load().kcg_kv_cache_read, device, cache._c, slots.data_ptr(), rk, rv, _DTYPES[dtype], B, slots.shape[-1])
+    return k, v
+
+
+def fmha_cache_workspace_bytes(cache, table_width, batch, drafts, heads):
+    """Bytes of workspace with which fmha_cache can split long sequences as it prefers to."""
+    _cache_check(cache)
+    return int(lib.load().kcg_fmha_cache_ws_bytes(cache._c, table_width, batch, drafts, heads))
+
+
+def fmha_cache(q, cache, block_table, context_lens, draft_lens=None, tree_mask=None, scale=1.0, out=None,
+               out_dtype=None, workspace=None):
+    """Attention of each sequence's newest tokens (one, a chain or a tree of drafts) over a cache.
+
+    q: bf16 [B,N,Hq,dim], N up to 64.  Sequence b has context_lens[b] keys that every query sees
+    and behind them those of its draft_lens[b] (default: N) drafted tokens, all already written;
+    block_table[b, j // page_size] is key j's page.  tree_mask: int64 [B,N], bit j of [b,n] says
+    that drafted token n sees drafted token j (default: a chain, j <= n).  Lengths and table are
+    int32.  Rows of `out` from draft_lens[b] on stay as they were.  kcg_fmha_cache says the rest.
+    """
+    device = _cache_check(cache)
+    if not isinstance(q, torch.Tensor) or q.dim() != 4:
+        raise ValueError("q must be a [B,N,H,dim] tensor")
+    rq = _rows(q, "q", torch.bfloat16, device)
+    B, N, Hq, D = q.shape
+    if D != cache.dim or Hq % cache.heads:
+        raise ValueError("q must have the cache's dim and a multiple of its heads")
+    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
+        raise ValueError("block_table must be an int32 tensor [B, pages]")
+    width = block_table.shape[1]
+    _check(block_table, "block_table", torch.int32, (B, width), device)
+    _check(context_lens, "context_lens", torch.int32, (B,), device)
+    if draft_lens is not None:
+        _check(draft_lens, "draft_lens", torch.int32, (B,), device)
+    if tree_mask is not None:
+        _check(tree_mask, "tree_mask", torch.int64, (B, N), device)
+    if out is None:
+        if draft_lens is not None:
+            out = torch.zeros(q.shape, dtype=out_dtype or torch.bfloat16, device=device)
+        else:
+            out = torch.empty(q.shape, dtype=out_dtype or torch.bfloat16, device=device)
+    elif out_dtype not in (None, out.dtype):
+        raise ValueError("out must have dtype %s, not %s" % (out_dtype, out.dtype))
+    if out.dtype not in _DTYPES:
+        raise ValueError("attention over a cache writes bfloat16 or float32, not %s" % out.dtype)
+    ro = _rows(out, "out", out.dtype, device, q.shape)
+    L = lib.load()
+    need = L.kcg_fmha_cache_ws_bytes(cache._c, width, B, N, Hq)
+    ws = _workspace(workspace, need, device)
+    _call(L.kcg_fmha_cache, device, rq, cache._c, block_table.data_ptr(), width, context_lens.data_ptr(),
+          draft_lens.data_ptr() if draft_lens is not None else None,
+          tree_mask.data_ptr() if tree_mask is not None else None, ro, _DTYPES[out.dtype], B, N, Hq, scale,
+          ws.data_ptr() if ws is not None else None, _bytes(ws) if ws is not None else 0)
     return out

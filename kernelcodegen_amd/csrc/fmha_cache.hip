@@ -1,9 +1,44 @@
 // Attention of the newest tokens (one, a chain or a tree of drafts) over a paged cache.
 //
-//   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - m),  over the keys that the query sees.
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c q.k_j - m),  c = scale log2(e), over the keys that
+//   the query sees.
+//
+// Few queries read many keys, so the keys are what is split: into units of whole 32-key chunks, a unit
+// to a workgroup, and inside it a contiguous range of chunks to each of the four waves.  The N * Hq /
+// heads query rows that share a key head are the 32 or 64 columns of the wave's matrix products.
+//
+//  * Every wave streams its own chunks through a private ring of two LDS buffers with direct
+//    global -> LDS loads: nothing is shared before the end, so there is no barrier in the loop, a wave
+//    waits only for its own loads (vmcnt), and the next chunk is in flight while one is computed.
+//  * S^T = K . Q^T (v_mfma_f32_32x32x16_bf16): the A operand is K rows as ds_read_b128, e4m3 bytes
+//    becoming bf16 with the row's power of two in the conversion itself; B is Q, in registers.  A lane
+//    then holds one query and 16 of the 32 keys, which is the B operand of O^T += V^T . P^T as it
+//    stands.  V^T comes from V's natural rows by the transposing LDS reads (b8 or b16); V's powers of
+//    two go into P, where they cost nothing in precision.
+//  * The sum over d may run in any order, so an e4m3 lane takes the 16 bytes of one ds_read_b128 as
+//    two steps' worth of its row, and Q is loaded to match.
+//  * LDS rows are unpadded (a direct load fills 1024 consecutive bytes); 16-byte pieces sit at
+//    piece ^ swizzle(row), applied to the global address on loading and to the LDS address on
+//    reading, so that 16 lanes of a read hit 16 different 16-byte columns of the banks.
+//  * Only chunks that reach beyond the context, or touch a page that the cache does not have, look at
+//    masks.  There, V rows that nobody sees are zeroed in LDS (their weight is 0, and 0 * NaN is not),
+//    and values that are not finite are taken out of the product and added to the rows that see them.
+//  * How many chunks make a unit follows from the lengths, which are on the device: every wave sums
+//    them up and finds its unit (no host synchronisation, equal work for ragged batches).  A sequence
+//    that fits one unit is written at once; the others leave normalised partial outputs and the
+//    logarithms of their sums in the workspace, joined by a second launch.
 #include "kv_cache.h"
 
 namespace kcg {
+
+typedef __bf16 bf16x8_v __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4_v __attribute__((ext_vector_type(4)));
+typedef int int2_v __attribute__((ext_vector_type(2)));
+
+constexpr int kFcWaves = 4;
+constexpr int kFcChunk = 32;      // keys to a chunk
+constexpr int kFcMinChunks = 4;   // of a unit: one to a wave
+constexpr float kFcTau = 8.0f;    // log2 by which a maximum may lag behind before the sums are rescaled
 
 template <typename C>
 struct FmhaCacheArgs {
@@ -12,86 +47,659 @@ struct FmhaCacheArgs {
   KvCache<C> cache;
   const int32_t *table, *context, *drafts;
   const uint64_t *tree;
-  int B, N, Hq, width;
-  float scale;
+  float *partial;  // [unit][head][tile][rows][D], then the logarithms [unit][head][tile][rows]
+  int64_t logs;    // where those begin, in floats
+  int B, N, Hq, width, group, tiles, rows, want_units, max_units;
+  float q_sign, c;
+  bool vec;
 };
 
-// One wave to a query head of a token: D / 8 lanes to a key, so 512 / D keys at a time, each with a
-// running maximum, sum and output of its own that are joined at the end.
-template <typename C, typename O, int D, bool VEC>
-__global__ __launch_bounds__(256) void fmha_cache_kernel(const FmhaCacheArgs<C> a) {
-  constexpr int LANES = D / 8, PER = 64 / LANES;
+// Chunks to a unit, and which unit of which sequence number `unit` is.
+struct FcUnit {
+  int b, index, count, first;  // unit `index` of the `count` of sequence b; `first`: the number of its unit 0
+  int chunks_per_unit;
+  KvLens len;
+};
+
+template <typename C>
+__device__ __forceinline__ KvLens fc_lens(const FmhaCacheArgs<C> &a, int b) {
+  return kv_lens(a.context[b], a.drafts ? a.drafts[b] : a.N, a.N,
+                 static_cast<int64_t>(a.width) << a.cache.shape.log2_page);
+}
+
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m);
+  return x;
+}
+
+// Every wave does this for itself: the lengths of all sequences, 64 at a time.  Sequences without
+// queries have no unit, the others at least one.  With `unit` < 0 looks for sequence -1 - unit.
+template <typename C>
+__device__ __forceinline__ bool find_unit(const FmhaCacheArgs<C> &a, int unit, FcUnit &u) {
   const int lane = threadIdx.x & 63;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (item >= static_cast<int64_t>(a.B) * a.N * a.Hq) return;
-  const int h = static_cast<int>(item % a.Hq), n = static_cast<int>(item / a.Hq % a.N);
-  const int b = static_cast<int>(item / a.Hq / a.N);
-  const int page = 1 << a.cache.shape.log2_page;
-  const KvLens len = kv_lens(a.context[b], a.drafts ? a.drafts[b] : a.N, a.N, static_cast<int64_t>(a.width) * page);
-  if (n >= len.queries) return;
-  const uint64_t seen = kv_seen(a.tree, static_cast<int64_t>(b) * a.N + n, n, len.drafts);
-  const int head = h / (a.Hq / a.cache.shape.heads);
-  const int e0 = 8 * (lane % LANES);
-  float q[8], acc[8] = {}, m = -INFINITY, l = 0.0f;
-  load8<VEC>(a.q.at(b, n, h) + e0, q);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] *= a.scale;
-  for (int key = lane / LANES; key < len.context + len.drafts; key += PER) {
-    if (key >= len.context && !((seen >> (key - len.context)) & 1)) continue;
-    const int64_t row = kv_row(a.cache.shape, a.table[static_cast<int64_t>(b) * a.width + (key >> a.cache.shape.log2_page)],
-                               head, key & (page - 1));
-    if (row < 0) continue;
-    float k[8], v[8], s = 0.0f;
-    cache_load8(a.cache.k + row * D + e0, a.cache.k_exp + row, k);
-    cache_load8(a.cache.v + row * D + e0, a.cache.v_exp + row, v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s = __builtin_fmaf(q[j], k[j], s);
-    s = row_sum<LANES>(s);
-    const float top = fmaxf(m, s);
-    const float keep = top == -INFINITY ? 0.0f : expf(m - top);
-    const float p = s == -INFINITY ? 0.0f : expf(s - top);
-    l = l * keep + p;
-    m = top;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = acc[j] * keep + p * v[j];
+  int64_t total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    int chunks = 0;
+    if (b0 + lane < a.B) {
+      const KvLens l = fc_lens(a, b0 + lane);
+      if (l.queries) chunks = (l.context + l.drafts + kFcChunk - 1) / kFcChunk;
+    }
+    total += __builtin_amdgcn_readfirstlane(wave_sum(chunks));
   }
+  int64_t per = (total + a.want_units - 1) / a.want_units;
+  per = per < kFcMinChunks ? kFcMinChunks : per > (1 << 30) ? 1 << 30 : per;  // (no sequence has as many)
+  u.chunks_per_unit = static_cast<int>(per);
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    KvLens l = {0, 0, 0};
+    int units = 0;
+    if (b0 + lane < a.B) {
+      l = fc_lens(a, b0 + lane);
+      const int chunks = (l.context + l.drafts + kFcChunk - 1) / kFcChunk;
+      if (l.queries) units = chunks <= per ? 1 : (chunks + static_cast<int>(per) - 1) / static_cast<int>(per);
+    }
+    int upto = units;
 #pragma unroll
-  for (int step = LANES; step < 64; step *= 2) {
-    const float m2 = __shfl_xor(m, step), l2 = __shfl_xor(l, step);
-    const float top = fmaxf(m, m2);
-    const float c1 = m == -INFINITY ? 0.0f : expf(m - top), c2 = m2 == -INFINITY ? 0.0f : expf(m2 - top);
-    l = l * c1 + l2 * c2;
-    m = top;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = acc[j] * c1 + __shfl_xor(acc[j], step) * c2;
+    for (int m = 1; m < 64; m *= 2) {
+      const int other = __shfl_up(upto, m);
+      if (lane >= m) upto += other;
+    }
+    const bool mine = unit >= 0 ? units && unit >= before + upto - units && unit < before + upto : b0 + lane == -1 - unit;
+    const uint64_t found = __ballot(mine);
+    if (found) {
+      const int at = __builtin_ctzll(found);
+      u.b = b0 + at;
+      u.count = __builtin_amdgcn_readlane(units, at);
+      u.first = before + __builtin_amdgcn_readlane(upto, at) - u.count;
+      u.index = unit - u.first;
+      u.len.context = __builtin_amdgcn_readlane(l.context, at);
+      u.len.drafts = __builtin_amdgcn_readlane(l.drafts, at);
+      u.len.queries = __builtin_amdgcn_readlane(l.queries, at);
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
-  if (lane < LANES) {
-    const float r = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] *= r;
-    O *to = static_cast<O *>(a.out.data) + b * a.out.stride_b + n * a.out.stride_s + h * a.out.stride_h;
-    store8<VEC>(to + e0, acc);
+  return false;
+}
+
+// What a chunk looks like in LDS.  C: element of the cache.
+template <typename C, int D>
+struct FcTile {
+  static constexpr int kRow = D * static_cast<int>(sizeof(C));  // bytes
+  static constexpr int kPieces = kRow / 16;
+  static constexpr int kRowsPer256 = 16 / kPieces;
+  static constexpr int kRowsPerLoad = 64 / kPieces;             // one wave-wide direct load: 1024 bytes
+  static constexpr int kLoads = kFcChunk / kRowsPerLoad;
+  static constexpr int kBytes = kFcChunk * kRow;                // K, or V
+  static constexpr int kBuffer = 2 * kBytes + (sizeof(C) == 1 ? 256 : 0);  // K, V, exponents
+  static constexpr int kLoadsPerChunk = 2 * kLoads + (sizeof(C) == 1 ? 1 : 0);
+  static constexpr int kRing = 2 * kFcWaves * kBuffer;
+  static constexpr int kJoinRow = D + 4;                        // floats; padded
+  static constexpr int kJoin = kFcWaves * 32 * kJoinRow * 4;
+  static constexpr int kLds = kRing > kJoin ? kRing : kJoin;
+  static_assert(kRowsPerLoad <= 16, "a load stays inside a page");
+
+  // K: 16 consecutive rows, one piece each
+  static __device__ __forceinline__ int swizzle_k(int row) { return (row / kRowsPer256) % kPieces; }
+  // V: b8 reads 32 lanes wide take rows {0-3, 8-11} (+ 4, + 16) of two neighbouring pieces, b16 reads four
+  // rows of four
+  static __device__ __forceinline__ int swizzle_v(int row) {
+    if (sizeof(C) == 1) return kPieces == 8 ? 2 * ((row >> 1) & 1) + 4 * ((row >> 3) & 1) : 2 * ((row >> 3) & 1);
+    return 4 * ((row / kRowsPer256) & (kPieces / 4 - 1));
   }
+};
+
+__device__ __forceinline__ unsigned lds_address(const void *p) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void *)p));
+}
+
+// lane l's 4 bytes at `from` go to LDS byte address to + 4 * l
+__device__ __forceinline__ void direct_load_4B(const void *from, unsigned to) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  unsigned saved_m0;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %2, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved_m0)
+      : "s"(to), "v"(from)
+      : "memory");
+#endif
+}
+
+// 8 e4m3 bytes times a power of two, as bf16.
+__device__ __forceinline__ bf16x8_v to_bf16(unsigned lo, unsigned hi, float scale) {
+  const bf16_pair_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+  const bf16_pair_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const bf16_pair_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+  const bf16_pair_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+  return bf16x8_v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+__device__ __forceinline__ bool not_finite(uint8_t x) { return (x & 0x7f) == 0x7f; }
+__device__ __forceinline__ bool not_finite(uint16_t x) { return (x & 0x7f80) == 0x7f80; }
+
+// Q rows of the tile: 32 * QT columns of the products; TERMS: bf16 numbers that a weight is split over.
+// Two waves to a SIMD where the registers (or a bf16 chunk's LDS) allow it.
+template <typename C, int D, int QT, int TERMS>
+__global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || sizeof(C) == 2) ? 1 : 2)) void fmha_cache_kernel(const FmhaCacheArgs<C> a) {
+  using T = FcTile<C, D>;
+  constexpr bool E8 = sizeof(C) == 1;
+  constexpr int DT = D / 32, DS = D / 16;
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r32 = lane & 31, half = lane >> 5;
+
+  // tiles of one (unit, head) share its keys: they go to one XCD (workgroup w runs on XCD w % 8)
+  const int w = blockIdx.x;
+  const int tile = (w / kNumXcd) % a.tiles;
+  const int item = w / (kNumXcd * a.tiles) * kNumXcd + w % kNumXcd;
+  const int heads = a.cache.shape.heads;
+  const int unit = item / heads, head = item - unit * heads;
+  FcUnit u;
+  if (unit >= a.max_units || !find_unit(a, unit, u)) return;
+  const int b = u.b;
+  const int row0 = tile * 32 * QT;  // first query row; row = node * group + query head within the group
+  if (row0 >= u.len.queries * a.group) return;
+
+  // ---- this wave's chunks ----
+  const int keys = u.len.context + u.len.drafts;
+  const int chunks = (keys + kFcChunk - 1) / kFcChunk;
+  const int unit_begin = u.index * u.chunks_per_unit;
+  const int unit_end = min(chunks, unit_begin + u.chunks_per_unit);
+  const int per_wave = (unit_end - unit_begin + kFcWaves - 1) / kFcWaves;
+  const int begin = min(unit_end, unit_begin + wave * per_wave), end = min(unit_end, begin + per_wave);
+
+  // ---- Q ----
+  bf16x8_v q[QT][DS];
+  uint64_t seen[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int row = row0 + 32 * t + r32;
+    const int node = row / a.group, h = head * a.group + row - node * a.group;
+    const bool live = node < u.len.queries;
+    seen[t] = live ? kv_seen(a.tree, static_cast<int64_t>(b) * a.N + node, node, u.len.drafts) : 0;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      float x[8] = {};
+      const int d = E8 ? 32 * (s / 2) + 16 * half + 8 * (s % 2) : 16 * s + 8 * half;
+      if (live) {
+        const uint16_t *from = a.q.at(b, node, h) + d;
+        if (a.vec) load8<true>(from, x);
+        else load8<false>(from, x);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[t][s][j] = static_cast<__bf16>(x[j] * a.q_sign);
+    }
+  }
+
+  // ---- pages of this wave, 64 at a time in the lanes of a register ----
+  const int log2_page = a.cache.shape.log2_page;
+  const int32_t *table = a.table + static_cast<int64_t>(b) * a.width;
+  int page_base = 0, pages = 0;
+  auto load_pages = [&](int first) {
+    page_base = first;
+    pages = table[min(first + lane, a.width - 1)];
+  };
+  load_pages((begin * kFcChunk) >> log2_page);
+  // page of a key (not beyond the wave's last chunk), -1 if the cache does not have it
+  auto page_of = [&](int key) {
+    const int index = key >> log2_page;
+    if (index >= a.width) return -1;
+    if (index - page_base >= 64) load_pages(index);
+    const int p = __builtin_amdgcn_readlane(pages, index - page_base);
+    return p >= 0 && p < a.cache.shape.pages ? p : -1;
+  };
+
+  uint8_t *ring = lds + wave * 2 * T::kBuffer;
+  const unsigned ring_at = __builtin_amdgcn_readfirstlane(lds_address(ring));
+  // byte offsets of this lane's pieces from the first row of a load
+  const int load_row = lane / T::kPieces, load_pos = lane % T::kPieces;
+  unsigned off_k[T::kLoads], off_v[T::kLoads];
+#pragma unroll
+  for (int j = 0; j < T::kLoads; ++j) {
+    const int row = j * T::kRowsPerLoad + load_row;
+    off_k[j] = load_row * T::kRow + (load_pos ^ T::swizzle_k(row)) * 16;
+    off_v[j] = load_row * T::kRow + (load_pos ^ T::swizzle_v(row)) * 16;
+  }
+  int valid[2] = {0, 0};  // per buffer: bit g: the page of keys 16 g .. 16 g + 15 is the cache's
+  auto load_chunk = [&](int chunk, int buffer) {
+    const int key0 = chunk * kFcChunk;
+    const int p0 = page_of(key0), p1 = page_of(key0 + 16);
+    const int ok = (p0 >= 0 ? 1 : 0) | (p1 >= 0 ? 2 : 0);
+    if (buffer) valid[1] = ok;
+    else valid[0] = ok;
+    const int in_page = (1 << log2_page) - 1;
+    const int64_t base[2] = {kv_row(a.cache.shape, max(p0, 0), head, key0 & in_page),
+                             kv_row(a.cache.shape, max(p1, 0), head, (key0 + 16) & in_page)};
+    const unsigned to = ring_at + buffer * T::kBuffer;
+    // the buffer's last reads are done (their results are used), as far as the hardware is told
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < T::kLoads; ++j) {
+      const int first = j * T::kRowsPerLoad;
+      const int64_t row = base[first / 16] + first % 16;
+      direct_load_16B(a.cache.k + row * D, off_k[j], to + j * 1024);
+      direct_load_16B(a.cache.v + row * D, off_v[j], to + T::kBytes + j * 1024);
+    }
+    if constexpr (E8) {
+      // dwords 0-7: K's exponents, 8-15: V's (the other lanes repeat them)
+      const int i = lane & 7;
+      const uint8_t *from = (lane & 8 ? a.cache.v_exp : a.cache.k_exp) + (i < 4 ? base[0] : base[1]) + 4 * (i & 3);
+      direct_load_4B(from, to + 2 * T::kBytes);
+    }
+  };
+
+  float16_t acc[QT][DT];
+  float m[QT], l[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[t][i][e] = 0.0f;
+  }
+
+  // V: row and byte column of this lane's transposing reads, within 16 keys and 32 columns
+  const int l16 = lane & 15, side = (lane >> 4) & 1;
+  const int v_row = E8 ? 4 * half + ((l16 >> 1) & 3) + 8 * (l16 >> 3) : 4 * half + (l16 >> 2);
+  const int v_piece = E8 ? side : 2 * side + ((l16 & 3) >> 1);
+  const int v_at = v_row * T::kRow + (l16 & 1) * 8;
+
+  if (begin < end) load_chunk(begin, 0);
+  if (begin + 1 < end) load_chunk(begin + 1, 1);
+  for (int chunk = begin; chunk < end; ++chunk) {
+    const int buffer = (chunk - begin) & 1;
+    if (chunk + 1 < end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::kLoadsPerChunk) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const uint8_t *ks = ring + buffer * T::kBuffer;
+    uint8_t *vs = ring + buffer * T::kBuffer + T::kBytes;
+    const uint8_t *xs = vs + T::kBytes;
+
+    // ---- S^T = K . Q^T ----
+    float16_t s[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
+    if constexpr (E8) {
+      const float scale = exponent_to_scale(xs[r32]);
+#pragma unroll
+      for (int p = 0; p < D / 32; ++p) {
+        const uint4_t x = *reinterpret_cast<const uint4_t *>(ks + r32 * T::kRow + ((2 * p + half) ^ T::swizzle_k(r32)) * 16);
+        const bf16x8_v k0 = to_bf16(x[0], x[1], scale), k1 = to_bf16(x[2], x[3], scale);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k0, q[t][2 * p], s[t], 0, 0, 0);
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1, q[t][2 * p + 1], s[t], 0, 0, 0);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int p = 0; p < DS; ++p) {
+        const uint4_t x = *reinterpret_cast<const uint4_t *>(ks + r32 * T::kRow + ((2 * p + half) ^ T::swizzle_k(r32)) * 16);
+        const bf16x8_v k = __builtin_bit_cast(bf16x8_v, x);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[t][p], s[t], 0, 0, 0);
+      }
+    }
+
+    // ---- masks ----
+    const int key0 = chunk * kFcChunk;
+    const int ok = buffer ? valid[1] : valid[0];
+    if (key0 + kFcChunk > u.len.context || ok != 3) {
+      const unsigned there = (ok & 1 ? 0x0000ffffu : 0u) | (ok & 2 ? 0xffff0000u : 0u);
+      const int d0 = key0 - u.len.context;  // the first key's place among the drafts
+      unsigned vis[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        unsigned v;
+        if (d0 >= 0) v = d0 < 64 ? static_cast<unsigned>(seen[t] >> d0) : 0u;
+        else if (d0 > -32) v = static_cast<unsigned>(seen[t] << -d0) | ((1u << -d0) - 1);
+        else v = 0xffffffffu;
+        vis[t] = v & there;
+        const unsigned mine = vis[t] >> (4 * half);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!((mine >> (8 * (e / 4) + e % 4)) & 1)) s[t][e] = -INFINITY;
+      }
+      // keys that some query may see; the rows of the others are zeroed
+      const int left = keys - key0;
+      const unsigned some = (left >= 32 ? 0xffffffffu : (1u << left) - 1) & there;
+      unsigned bad = 0;  // rows with values that are not finite
+#pragma unroll 1
+      for (int j = 0; j < T::kLoads; ++j) {
+        const int row = j * T::kRowsPerLoad + load_row;
+        uint4_t *piece = reinterpret_cast<uint4_t *>(vs + j * 1024 + lane * 16);
+        uint4_t x = *piece;
+        bool any = false;
+        if (!((some >> row) & 1)) {
+          *piece = uint4_t{0, 0, 0, 0};
+        } else {
+#pragma unroll
+          for (int i = 0; i < static_cast<int>(16 / sizeof(C)); ++i)
+            any |= not_finite(static_cast<C>(x[i * sizeof(C) / 4] >> (8 * (i * sizeof(C) % 4))));
+        }
+        uint64_t where = __ballot(any);
+        while (where) {
+          const int at = __builtin_ctzll(where);
+          bad |= 1u << (j * T::kRowsPerLoad + at / T::kPieces);
+          where &= where - 1;
+        }
+      }
+      if (bad) {  // (uniform)
+        for (unsigned left_over = bad; left_over; left_over &= left_over - 1) {
+          const int row = __builtin_ctz(left_over);
+#pragma unroll
+          for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int byte = (32 * i + 8 * (e / 4) + 4 * half + e % 4) * static_cast<int>(sizeof(C));
+              const C x = *reinterpret_cast<const C *>(vs + row * T::kRow + ((byte / 16) ^ T::swizzle_v(row)) * 16 + byte % 16);
+              if (not_finite(x)) {
+                const float y = E8 ? NAN : bf16_to_float(static_cast<uint16_t>(x));
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+                  if ((vis[t] >> row) & 1) acc[t][i][e] += y;
+              }
+            }
+        }
+#pragma unroll 1
+        for (int j = 0; j < T::kLoads; ++j) {
+          C *piece = reinterpret_cast<C *>(vs + j * 1024 + lane * 16);
+#pragma unroll 1
+          for (int i = 0; i < static_cast<int>(16 / sizeof(C)); ++i)
+            if (not_finite(piece[i])) piece[i] = 0;
+        }
+      }
+    }
+
+    // ---- weights ----
+    unsigned p[QT][TERMS][8];  // bf16 pairs: elements 2w, 2w + 1
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      // The first maximum is the compiler's: it knows how long a product's result takes, the assembly
+      // of max3 does not, and each max3 needs the one before.
+      float top = fmaxf(s[t][0], s[t][1]);
+#pragma unroll
+      for (int e = 2; e < 16; e += 2) top = max3(top, s[t][e], s[t][e + 1]);
+      top *= a.c;
+      top = max_across_halves(top);
+      if (top > m[t] + kFcTau) {
+        const float keep = __builtin_amdgcn_exp2f(m[t] - top);  // 0 the first time
+        m[t] = top;
+        l[t] *= keep;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[t][i][e] *= keep;
+      }
+      const float neg = m[t] == -INFINITY ? 0.0f : -m[t];
+      unsigned x[4] = {};
+      if constexpr (E8) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)  // V's exponents of the keys 8 g + 4 half .. + 3, less 128
+          x[g] = *reinterpret_cast<const unsigned *>(xs + 32 + 8 * g + 4 * half) ^ 0x80808080u;
+      }
+#pragma unroll
+      for (int w2 = 0; w2 < 8; ++w2) {
+        float y[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) y[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][2 * w2 + k], a.c, neg));
+        if (TERMS == 1) {
+          // the sum of the weights as they are rounded: what rounding does to one key alone cancels
+          const bf16_pair_t ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+          l[t] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16_pair_t, float_to_bf16_pair(y[0], y[1])), ones,
+                                                 l[t], false);
+        } else {
+          l[t] += y[0] + y[1];
+        }
+        if constexpr (E8) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int e = 2 * w2 + k;
+            y[k] = __builtin_ldexpf(y[k], static_cast<int>(x[e / 4] << (24 - 8 * (e % 4))) >> 24);
+          }
+        }
+#pragma unroll
+        for (int z = 0; z < TERMS; ++z) {
+          const unsigned pair = float_to_bf16_pair(y[0], y[1]);
+          p[t][z][w2] = pair;
+          y[0] -= __builtin_bit_cast(float, pair << 16);
+          y[1] -= __builtin_bit_cast(float, pair & 0xffff0000u);
+        }
+      }
+    }
+
+    // ---- O^T += V^T . P^T ----
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < DT; ++i) {
+        bf16x8_v v;
+        if constexpr (E8) {
+          const int piece = (2 * i + v_piece) ^ T::swizzle_v(v_row);  // rows 16 apart have one swizzle
+          const int2_v x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (__attribute__((address_space(3))) int2_v *)(vs + kb * 16 * T::kRow + v_at + piece * 16));
+          v = to_bf16(static_cast<unsigned>(x[0]), static_cast<unsigned>(x[1]), 1.0f);
+        } else {
+          const int piece = (4 * i + v_piece) ^ T::swizzle_v(v_row);  // rows 8 and 16 apart have one swizzle
+          const uint8_t *from = vs + kb * 16 * T::kRow + v_at + piece * 16;
+          const bf16x4_v lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4_v *)from);
+          const bf16x4_v hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+              (__attribute__((address_space(3))) bf16x4_v *)(from + 8 * T::kRow));
+          v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int z = 0; z < TERMS; ++z) {
+            const uint4_t y = {p[t][z][4 * kb], p[t][z][4 * kb + 1], p[t][z][4 * kb + 2], p[t][z][4 * kb + 3]};
+            acc[t][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8_v, y), acc[t][i], 0, 0, 0);
+          }
+      }
+    if (chunk + 2 < end) load_chunk(chunk + 2, buffer);
+  }
+
+  // ---- join the waves ----
+  float *join = reinterpret_cast<float *>(lds);
+  __shared__ float stats[2][kFcWaves][32 * QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    l[t] += __shfl_xor(l[t], 32);
+    if (half == 0) {
+      stats[0][wave][32 * t + r32] = m[t];
+      stats[1][wave][32 * t + r32] = l[t];
+    }
+  }
+  const bool whole = u.count == 1;
+  const int64_t slot = (static_cast<int64_t>(unit) * heads + head) * a.tiles + tile;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    __syncthreads();  // statistics are there; ring buffers and the last round's outputs are done with
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kFcWaves; ++k) top = fmaxf(top, stats[0][k][32 * t + r32]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int k = 0; k < kFcWaves; ++k)
+      sum += stats[1][k][32 * t + r32] * __builtin_amdgcn_exp2f(stats[0][k][32 * t + r32] - ref);
+    // (e4m3: the weights were 2^-1 of what they stand for)
+    const float norm = (sum == 0.0f ? 0.0f : (E8 ? 2.0f : 1.0f) / sum) * __builtin_amdgcn_exp2f(m[t] - ref);
+    float *mine = join + (wave * 32 + r32) * T::kJoinRow + 4 * half;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float16_t &x = acc[t][i];
+        *reinterpret_cast<float4_t *>(mine + 32 * i + 8 * g) =
+            float4_t{x[4 * g] * norm, x[4 * g + 1] * norm, x[4 * g + 2] * norm, x[4 * g + 3] * norm};
+      }
+    const int row = 32 * t + r32;
+    if (!whole && wave == 0 && half == 0 && row < a.rows)
+      a.partial[a.logs + slot * a.rows + row] = sum == 0.0f ? -INFINITY : ref + __builtin_amdgcn_logf(sum);
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * (D / 4); i += 64 * kFcWaves) {
+      const int r = i / (D / 4), d = 4 * (i % (D / 4));
+      const int at = row0 + 32 * t + r, node = at / a.group, h = head * a.group + at - node * a.group;
+      if (node >= u.len.queries) break;
+      float4_t y = {};
+#pragma unroll
+      for (int k = 0; k < kFcWaves; ++k) y += *reinterpret_cast<const float4_t *>(join + (k * 32 + r) * T::kJoinRow + d);
+      if (!whole) {
+        *reinterpret_cast<float4_t *>(a.partial + (slot * a.rows + 32 * t + r) * D + d) = y;
+      } else if constexpr (TERMS == 1) {
+        uint16_t *to = static_cast<uint16_t *>(a.out.data) + b * a.out.stride_b + node * a.out.stride_s + h * a.out.stride_h + d;
+        const uint2_t z = {float_to_bf16_pair(y[0], y[1]), float_to_bf16_pair(y[2], y[3])};
+        if (a.vec) *reinterpret_cast<uint2_t *>(to) = z;
+        else
+          for (int j = 0; j < 4; ++j) to[j] = float_to_bf16(y[j]);
+      } else {
+        float *to = static_cast<float *>(a.out.data) + b * a.out.stride_b + node * a.out.stride_s + h * a.out.stride_h + d;
+        if (a.vec) *reinterpret_cast<float4_t *>(to) = y;
+        else
+          for (int j = 0; j < 4; ++j) to[j] = y[j];
+      }
+    }
+  }
+}
+
+// Joins the units of the sequences that have several: a wave to an output row.
+template <typename C, int D, typename O>
+__global__ __launch_bounds__(256) void fmha_cache_join_kernel(const FmhaCacheArgs<C> a) {
+  constexpr int PER = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int rows = a.N * a.Hq;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = static_cast<int>(item / rows);
+  if (b >= a.B) return;
+  const int at = static_cast<int>(item - static_cast<int64_t>(b) * rows);
+  const int node = at / a.Hq, h = at - node * a.Hq;
+  FcUnit u;
+  if (!find_unit(a, -1 - b, u) || u.count < 2 || node >= u.len.queries) return;
+  const int head = h / a.group, row = node * a.group + h - head * a.group;
+  const int per_tile = a.tiles == 1 ? a.rows : 64;
+  const int tile = row / per_tile, r = row - tile * per_tile;
+  const int64_t step = static_cast<int64_t>(a.cache.shape.heads) * a.tiles * a.rows;
+  const int64_t first = (static_cast<int64_t>(u.first) * a.cache.shape.heads + head) * a.tiles * a.rows +
+                        static_cast<int64_t>(tile) * a.rows + r;
+  float top = -INFINITY;
+  for (int i = lane; i < u.count; i += 64) top = fmaxf(top, a.partial[a.logs + first + i * step]);
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f, y[PER] = {};
+#pragma unroll 4
+  for (int i = 0; i < u.count; ++i) {
+    const float weight = __builtin_amdgcn_exp2f(a.partial[a.logs + first + i * step] - ref);
+    const float *from = a.partial + (first + i * step) * D + lane * PER;
+    sum += weight;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) y[j] += weight * from[j];
+  }
+  O *to = static_cast<O *>(a.out.data) + b * a.out.stride_b + node * a.out.stride_s + h * a.out.stride_h + lane * PER;
+  const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if constexpr (sizeof(O) == 2) to[j] = float_to_bf16(y[j] * norm);
+    else to[j] = y[j] * norm;
+  }
+}
+
+// How a call is split; the query and the call agree on it.
+struct FcPlan {
+  int group, rows_all, qt, tiles, rows;  // rows: of a tile that are stored
+  int want_units, max_units;
+  int64_t floats;  // workspace
+};
+
+inline FcPlan plan_fmha_cache(const kcg_kv_cache &c, int width, int B, int N, int Hq, int64_t workspace_bytes) {
+  FcPlan p;
+  p.group = Hq / c.heads;
+  p.rows_all = N * p.group;
+  p.qt = p.rows_all <= 32 ? 1 : 2;
+  p.tiles = (p.rows_all + 32 * p.qt - 1) / (32 * p.qt);
+  p.rows = p.tiles > 1 ? 64 : p.rows_all;
+  const int64_t per_unit = static_cast<int64_t>(c.heads) * p.tiles;
+  // units so that there are some workgroups to each of the CU's two places
+  int64_t want = (2048 + per_unit - 1) / per_unit;
+  const int64_t chunks = (static_cast<int64_t>(width) * c.page_size + kFcChunk - 1) / kFcChunk;
+  const int64_t most = B * ((chunks + kFcMinChunks - 1) / kFcMinChunks);
+  if (want > most) want = most;
+  const int64_t floats_per_unit = per_unit * p.rows * (c.dim + 1);
+  int64_t units = want + B;
+  if (workspace_bytes >= 0 && units > workspace_bytes / 4 / floats_per_unit) units = workspace_bytes / 4 / floats_per_unit;
+  if (chunks <= kFcMinChunks || units <= B) {
+    // one unit to a sequence: nothing is stored between
+    p.want_units = 0;
+    p.max_units = B;
+    p.floats = 0;
+    return p;
+  }
+  p.want_units = static_cast<int>(units - B);
+  p.max_units = static_cast<int>(units);
+  p.floats = units * floats_per_unit;
+  return p;
+}
+
+template <typename C, int D, int QT, int TERMS>
+int run_fmha_cache(FmhaCacheArgs<C> &a, bool split, hipStream_t stream) {
+  const auto kernel = fmha_cache_kernel<C, D, QT, TERMS>;
+  const int lds = FcTile<C, D>::kLds;
+  if (!allow_lds(kernel, lds)) return KCG_ERR_LAUNCH;
+  const int64_t items = static_cast<int64_t>(a.max_units) * a.cache.shape.heads;
+  const int64_t grid = (items + kNumXcd - 1) / kNumXcd * kNumXcd * a.tiles;
+  if (grid > 0x7fffffffLL) return KCG_ERR_UNSUPPORTED_SHAPE;
+  if (const int e = launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * kFcWaves), lds, stream, a)) return e;
+  if (!split) return KCG_OK;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.N * a.Hq;
+  using O = std::conditional_t<TERMS == 1, uint16_t, float>;
+  return launch(fmha_cache_join_kernel<C, D, O>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream, a);
 }
 
 template <typename C>
 int fmha_cache(const kcg_rows &q, const kcg_kv_cache &cache, const int32_t *table, int width, const int32_t *context,
                const int32_t *drafts, const uint64_t *tree, const kcg_rows &out, int o_dtype, int B, int N, int Hq,
-               float scale, hipStream_t stream) {
-  FmhaCacheArgs<C> a = {make_rows<const uint16_t>(q), make_rows<void>(out), make_cache<C>(cache), table, context, drafts, tree, B, N, Hq, width, scale};
-  const bool vec = rows_aligned16(q, KCG_BF16, B, N, Hq) && rows_aligned16(out, o_dtype, B, N, Hq);
-  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(B) * N * Hq + 3) / 4));
-#define KCG_PICK(O, DD, V) return launch(fmha_cache_kernel<C, O, DD, V>, grid, dim3(256), 0, stream, a)
-#define KCG_PICK2(O)                     \
-  if (cache.dim == 64) {                 \
-    if (vec) { KCG_PICK(O, 64, true); }  \
-    KCG_PICK(O, 64, false);              \
-  }                                      \
-  if (vec) { KCG_PICK(O, 128, true); }   \
-  KCG_PICK(O, 128, false)
-  if (o_dtype == KCG_F32) { KCG_PICK2(float); }
-  KCG_PICK2(uint16_t);
-#undef KCG_PICK2
+               float scale, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
+  const FcPlan p = plan_fmha_cache(cache, width, B, N, Hq, workspace ? workspace_bytes : 0);
+  const bool split = p.want_units > 0;
+  FmhaCacheArgs<C> a = {};
+  a.q = make_rows<const uint16_t>(q);
+  a.out = make_rows<void>(out);
+  a.cache = make_cache<C>(cache);
+  a.table = table;
+  a.context = context;
+  a.drafts = drafts;
+  a.tree = tree;
+  a.partial = static_cast<float *>(workspace);
+  a.logs = static_cast<int64_t>(p.max_units) * cache.heads * p.tiles * p.rows * cache.dim;
+  a.B = B;
+  a.N = N;
+  a.Hq = Hq;
+  a.width = width;
+  a.group = p.group;
+  a.tiles = p.tiles;
+  a.rows = p.rows;
+  a.want_units = split ? p.want_units : 1;
+  a.max_units = p.max_units;
+  // the scale's sign goes into Q, so that the maximum of the scores is that of the products
+  a.q_sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;
+  a.c = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504088896340736f;
+  a.vec = rows_aligned16(q, KCG_BF16, B, N, Hq) && rows_aligned16(out, o_dtype, B, N, Hq);
+#define KCG_PICK(DD, QQ) \
+  return o_dtype == KCG_F32 ? run_fmha_cache<C, DD, QQ, 3>(a, split, stream) : run_fmha_cache<C, DD, QQ, 1>(a, split, stream)
+  if (cache.dim == 64) {
+    if (p.qt == 1) { KCG_PICK(64, 1); }
+    KCG_PICK(64, 2);
+  }
+  if (p.qt == 1) { KCG_PICK(128, 1); }
+  KCG_PICK(128, 2);
 #undef KCG_PICK
 }
 
@@ -100,7 +708,7 @@ inline int check_fmha_cache(const kcg_kv_cache *cache, int64_t width, int64_t B,
   if (const int e = check_cache(cache)) return e;
   if (width <= 0 || B <= 0 || N <= 0 || Hq <= 0) return KCG_ERR_BAD_SHAPE;
   if (N > 64 || Hq % cache->heads) return KCG_ERR_UNSUPPORTED_SHAPE;
-  if (width > 0x7fffffffLL / cache->page_size || B > 0x7fffffffLL / width) return KCG_ERR_UNSUPPORTED_SHAPE;
+  if (width > 0x7fffff00LL / cache->page_size || B > 0x7fffffffLL / width) return KCG_ERR_UNSUPPORTED_SHAPE;
   return check_extents(B, N, Hq, cache->dim);
 }
 
@@ -109,8 +717,8 @@ inline int check_fmha_cache(const kcg_kv_cache *cache, int64_t width, int64_t B,
 extern "C" {
 
 int64_t kcg_fmha_cache_ws_bytes(const kcg_kv_cache *cache, int32_t table_width, int32_t B, int32_t N, int32_t Hq) {
-  (void)cache, (void)table_width, (void)B, (void)N, (void)Hq;
-  return 0;
+  if (kcg::check_fmha_cache(cache, table_width, B, N, Hq)) return 0;
+  return kcg::plan_fmha_cache(*cache, table_width, B, N, Hq, -1).floats * 4;
 }
 
 int kcg_fmha_cache(const kcg_rows *q, const kcg_kv_cache *cache, const int32_t *block_table, int32_t table_width,
@@ -129,9 +737,9 @@ int kcg_fmha_cache(const kcg_rows *q, const kcg_kv_cache *cache, const int32_t *
   hipStream_t st = static_cast<hipStream_t>(stream);
   return cache->dtype == KCG_E4M3
              ? kcg::fmha_cache<uint8_t>(*q, *cache, block_table, table_width, context_lens, draft_lens, tree_mask, *out,
-                                        o_dtype, B, N, Hq, scale, st)
+                                        o_dtype, B, N, Hq, scale, workspace, workspace_bytes, st)
              : kcg::fmha_cache<uint16_t>(*q, *cache, block_table, table_width, context_lens, draft_lens, tree_mask, *out,
-                                         o_dtype, B, N, Hq, scale, st);
+                                         o_dtype, B, N, Hq, scale, workspace, workspace_bytes, st);
 }
 
 }  // extern "C"

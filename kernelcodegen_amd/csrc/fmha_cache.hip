@@ -79,12 +79,11 @@ template <typename C>
 __device__ __forceinline__ bool find_unit(const FmhaCacheArgs<C> &a, int unit, FcUnit &u) {
   const int lane = threadIdx.x & 63;
   int64_t total = 0;
+  KvLens l = {0, 0, 0};
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    int chunks = 0;
-    if (b0 + lane < a.B) {
-      const KvLens l = fc_lens(a, b0 + lane);
-      if (l.queries) chunks = (l.context + l.drafts + kFcChunk - 1) / kFcChunk;
-    }
+    l = {0, 0, 0};
+    if (b0 + lane < a.B) l = fc_lens(a, b0 + lane);
+    const int chunks = l.queries ? (l.context + l.drafts + kFcChunk - 1) / kFcChunk : 0;
     total += __builtin_amdgcn_readfirstlane(wave_sum(chunks));
   }
   int64_t per = (total + a.want_units - 1) / a.want_units;
@@ -92,13 +91,12 @@ __device__ __forceinline__ bool find_unit(const FmhaCacheArgs<C> &a, int unit, F
   u.chunks_per_unit = static_cast<int>(per);
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    KvLens l = {0, 0, 0};
-    int units = 0;
-    if (b0 + lane < a.B) {
-      l = fc_lens(a, b0 + lane);
-      const int chunks = (l.context + l.drafts + kFcChunk - 1) / kFcChunk;
-      if (l.queries) units = chunks <= per ? 1 : (chunks + static_cast<int>(per) - 1) / static_cast<int>(per);
+    if (a.B > 64) {  // (else they are still there)
+      l = {0, 0, 0};
+      if (b0 + lane < a.B) l = fc_lens(a, b0 + lane);
     }
+    const int chunks = (l.context + l.drafts + kFcChunk - 1) / kFcChunk;
+    const int units = !l.queries ? 0 : chunks <= per ? 1 : (chunks + static_cast<int>(per) - 1) / static_cast<int>(per);
     int upto = units;
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) {
@@ -214,29 +212,6 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
   const int per_wave = (unit_end - unit_begin + kFcWaves - 1) / kFcWaves;
   const int begin = min(unit_end, unit_begin + wave * per_wave), end = min(unit_end, begin + per_wave);
 
-  // ---- Q ----
-  bf16x8_v q[QT][DS];
-  uint64_t seen[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int row = row0 + 32 * t + r32;
-    const int node = row / a.group, h = head * a.group + row - node * a.group;
-    const bool live = node < u.len.queries;
-    seen[t] = live ? kv_seen(a.tree, static_cast<int64_t>(b) * a.N + node, node, u.len.drafts) : 0;
-#pragma unroll
-    for (int s = 0; s < DS; ++s) {
-      float x[8] = {};
-      const int d = E8 ? 32 * (s / 2) + 16 * half + 8 * (s % 2) : 16 * s + 8 * half;
-      if (live) {
-        const uint16_t *from = a.q.at(b, node, h) + d;
-        if (a.vec) load8<true>(from, x);
-        else load8<false>(from, x);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) q[t][s][j] = static_cast<__bf16>(x[j] * a.q_sign);
-    }
-  }
-
   // ---- pages of this wave, 64 at a time in the lanes of a register ----
   const int log2_page = a.cache.shape.log2_page;
   const int32_t *table = a.table + static_cast<int64_t>(b) * a.width;
@@ -244,6 +219,9 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
   auto load_pages = [&](int first) {
     page_base = first;
     pages = table[min(first + lane, a.width - 1)];
+    // has it arrive here: a load that may still be under way at the next use would make every use wait
+    // for all loads, those of the chunks ahead among them
+    asm volatile("" ::"v"(pages));
   };
   load_pages((begin * kFcChunk) >> log2_page);
   // page of a key (not beyond the wave's last chunk), -1 if the cache does not have it
@@ -294,6 +272,43 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
     }
   };
 
+  if (begin < end) load_chunk(begin, 0);
+  if (begin + 1 < end) load_chunk(begin + 1, 1);
+
+  // ---- Q ----
+  // The last QL steps of Q are kept in LDS where the accumulators of two tiles leave no registers for them.
+  constexpr int QL = D * QT == 256 && E8 && TERMS == 1 ? 4 : 0;
+  __shared__ uint4_t q_lds[QL ? QT : 1][QL ? QL : 1][QL ? 64 : 1];
+  bf16x8_v q[QT][DS - QL];
+  uint64_t seen[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int row = row0 + 32 * t + r32;
+    const int node = row / a.group, h = head * a.group + row - node * a.group;
+    const bool live = node < u.len.queries;
+    seen[t] = live ? kv_seen(a.tree, static_cast<int64_t>(b) * a.N + node, node, u.len.drafts) : 0;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      float x[8] = {};
+      const int d = E8 ? 32 * (s / 2) + 16 * half + 8 * (s % 2) : 16 * s + 8 * half;
+      if (live) {
+        const uint16_t *from = a.q.at(b, node, h) + d;
+        if (a.vec) load8<true>(from, x);
+        else load8<false>(from, x);
+      }
+      bf16x8_v y;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = static_cast<__bf16>(x[j] * a.q_sign);
+      if (s < DS - QL) q[t][s] = y;
+      else if (wave == s - (DS - QL)) q_lds[QL ? t : 0][QL ? s - (DS - QL) : 0][QL ? lane : 0] = __builtin_bit_cast(uint4_t, y);
+    }
+  }
+  if (QL) __syncthreads();
+  auto q_of = [&](int t, int s) {
+    return s < DS - QL ? q[t][s < DS - QL ? s : 0]
+                       : __builtin_bit_cast(bf16x8_v, q_lds[QL ? t : 0][QL ? s - (DS - QL) : 0][QL ? lane : 0]);
+  };
+
   float16_t acc[QT][DT];
   float m[QT], l[QT];
 #pragma unroll
@@ -312,8 +327,6 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
   const int v_piece = E8 ? side : 2 * side + ((l16 & 3) >> 1);
   const int v_at = v_row * T::kRow + (l16 & 1) * 8;
 
-  if (begin < end) load_chunk(begin, 0);
-  if (begin + 1 < end) load_chunk(begin + 1, 1);
   for (int chunk = begin; chunk < end; ++chunk) {
     const int buffer = (chunk - begin) & 1;
     if (chunk + 1 < end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::kLoadsPerChunk) : "memory");
@@ -336,8 +349,8 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
         const bf16x8_v k0 = to_bf16(x[0], x[1], scale), k1 = to_bf16(x[2], x[3], scale);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k0, q[t][2 * p], s[t], 0, 0, 0);
-          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1, q[t][2 * p + 1], s[t], 0, 0, 0);
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k0, q_of(t, 2 * p), s[t], 0, 0, 0);
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k1, q_of(t, 2 * p + 1), s[t], 0, 0, 0);
         }
       }
     } else {
@@ -346,7 +359,7 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
         const uint4_t x = *reinterpret_cast<const uint4_t *>(ks + r32 * T::kRow + ((2 * p + half) ^ T::swizzle_k(r32)) * 16);
         const bf16x8_v k = __builtin_bit_cast(bf16x8_v, x);
 #pragma unroll
-        for (int t = 0; t < QT; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[t][p], s[t], 0, 0, 0);
+        for (int t = 0; t < QT; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q_of(t, p), s[t], 0, 0, 0);
       }
     }
 
@@ -570,45 +583,57 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
   }
 }
 
-// Joins the units of the sequences that have several: a wave to an output row.
+// Joins the units of the sequences that have several: a workgroup to an output row, D / 4 lanes of
+// float4 to a unit's share of it, so that 1024 / D units are on their way at a time.
 template <typename C, int D, typename O>
 __global__ __launch_bounds__(256) void fmha_cache_join_kernel(const FmhaCacheArgs<C> a) {
-  constexpr int PER = D / 64;
+  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+  __shared__ float4_t shares[GROUPS][LANES];
+  __shared__ float sums[GROUPS];
   const int lane = threadIdx.x & 63;
-  const int rows = a.N * a.Hq;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = static_cast<int>(item / rows);
-  if (b >= a.B) return;
-  const int at = static_cast<int>(item - static_cast<int64_t>(b) * rows);
+  const int per_sequence = a.N * a.Hq;
+  const int b = blockIdx.x / per_sequence, at = blockIdx.x - b * per_sequence;
   const int node = at / a.Hq, h = at - node * a.Hq;
   FcUnit u;
   if (!find_unit(a, -1 - b, u) || u.count < 2 || node >= u.len.queries) return;
   const int head = h / a.group, row = node * a.group + h - head * a.group;
-  const int per_tile = a.tiles == 1 ? a.rows : 64;
-  const int tile = row / per_tile, r = row - tile * per_tile;
+  const int tile = a.tiles == 1 ? 0 : row / 64, r = row - tile * 64;
   const int64_t step = static_cast<int64_t>(a.cache.shape.heads) * a.tiles * a.rows;
   const int64_t first = (static_cast<int64_t>(u.first) * a.cache.shape.heads + head) * a.tiles * a.rows +
                         static_cast<int64_t>(tile) * a.rows + r;
+  const float *logs = a.partial + a.logs + first;
+  const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
+  // the first shares are on their way while the logarithms are looked through
+  float4_t y = {}, next = {};
+  if (group < u.count) next = *reinterpret_cast<const float4_t *>(a.partial + (first + group * step) * D + d);
   float top = -INFINITY;
-  for (int i = lane; i < u.count; i += 64) top = fmaxf(top, a.partial[a.logs + first + i * step]);
+  for (int i = lane; i < u.count; i += 64) top = fmaxf(top, logs[i * step]);
 #pragma unroll
   for (int k = 1; k < 64; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
   const float ref = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f, y[PER] = {};
-#pragma unroll 4
-  for (int i = 0; i < u.count; ++i) {
-    const float weight = __builtin_amdgcn_exp2f(a.partial[a.logs + first + i * step] - ref);
-    const float *from = a.partial + (first + i * step) * D + lane * PER;
+  float sum = 0.0f;
+  for (int i = group; i < u.count; i += GROUPS) {
+    const float4_t x = next;
+    if (i + GROUPS < u.count) next = *reinterpret_cast<const float4_t *>(a.partial + (first + (i + GROUPS) * step) * D + d);
+    const float weight = __builtin_amdgcn_exp2f(logs[i * step] - ref);
     sum += weight;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) y[j] += weight * from[j];
+    for (int j = 0; j < 4; ++j) y[j] = __builtin_fmaf(weight, x[j], y[j]);
   }
-  O *to = static_cast<O *>(a.out.data) + b * a.out.stride_b + node * a.out.stride_s + h * a.out.stride_h + lane * PER;
-  const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
+  shares[group][threadIdx.x % LANES] = y;
+  if (d == 0) sums[group] = sum;
+  __syncthreads();
+  if (group) return;
+  for (int k = 1; k < GROUPS; ++k) {  // (in a fixed order)
+    y += shares[k][threadIdx.x];
+    sum += sums[k];
+  }
+  y *= sum == 0.0f ? 0.0f : 1.0f / sum;
+  O *to = static_cast<O *>(a.out.data) + b * a.out.stride_b + node * a.out.stride_s + h * a.out.stride_h + d;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    if constexpr (sizeof(O) == 2) to[j] = float_to_bf16(y[j] * norm);
-    else to[j] = y[j] * norm;
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(O) == 2) to[j] = float_to_bf16(y[j]);
+    else to[j] = y[j];
   }
 }
 
@@ -660,7 +685,7 @@ int run_fmha_cache(FmhaCacheArgs<C> &a, bool split, hipStream_t stream) {
   if (!split) return KCG_OK;
   const int64_t rows = static_cast<int64_t>(a.B) * a.N * a.Hq;
   using O = std::conditional_t<TERMS == 1, uint16_t, float>;
-  return launch(fmha_cache_join_kernel<C, D, O>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream, a);
+  return launch(fmha_cache_join_kernel<C, D, O>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, a);
 }
 
 template <typename C>

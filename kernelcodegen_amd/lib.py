@@ -6,6 +6,7 @@ torch is used for device memory and streams only.
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # KCG_LIBRARY names another build of the same library (the experiment builds of
@@ -41,6 +42,11 @@ class Rows(ctypes.Structure):
     _fields_ = [("data", _vp), ("stride_b", _i64), ("stride_s", _i64), ("stride_h", _i64)]
 
 
+# kcg_rows as the bytes of its four members: what an entry point is handed by address, at a third of
+# the time that a ctypes structure takes
+pack_rows = struct.Struct("Pqqq").pack
+
+
 class KvCache(ctypes.Structure):
     """kcg_kv_cache: a paged key/value cache."""
     _fields_ = [("k", _vp), ("v", _vp), ("k_exp", _vp), ("v_exp", _vp), ("dtype", _i32), ("pages", _i32),
@@ -55,7 +61,7 @@ class LaunchInfo(ctypes.Structure):
                 ("tail_kernel", ctypes.c_char * 64)]
 
 
-_rows = ctypes.POINTER(Rows)
+_rows = _vp  # const kcg_rows *: pack_rows(...), or byref(Rows(...))
 _cache = ctypes.POINTER(KvCache)
 
 # name -> (restype, argtypes); every symbol include/kcg.h declares.
@@ -125,6 +131,14 @@ def check(status):
         raise KcgError(status, status_str(status))
 
 
+def raw_stream(index):
+    """The current stream of device `index` as a number.  (torch.cuda.current_stream builds a
+    Stream object for it, which takes as long as a small kernel.)"""
+    import torch
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return get(index) if get is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def current_stream():
     import torch
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return ctypes.c_void_p(raw_stream(torch.cuda.current_device()))

@@ -185,64 +185,82 @@ def fmha(Q, K, V, scale=1.0, causal=False, out=None, out_dtype=None, sched=None)
 # ---- attention layers that serve --------------------------------------------------------
 
 
-def _rows(t, name, dtype, device, shape=None):
-    """A [B,S,H,D] (or [tokens,H,D]) tensor with any strides but a contiguous last axis."""
+# A small call takes as long as its checks: each helper below first asks everything in one
+# expression and looks for what is wrong only where that fails.
+
+
+def _rows(t, name, dtype, index, shape=None):
+    """kcg_rows of a [B,S,H,D] (or [tokens,H,D]) tensor on device `index`: any strides but a
+    contiguous last axis."""
+    if isinstance(t, torch.Tensor) and t.dtype == dtype and t.get_device() == index and (
+            shape is None or t.shape == shape):
+        stride = t.stride()
+        if len(stride) == 4 and stride[3] == 1:
+            return lib.pack_rows(t.data_ptr(), stride[0], stride[1], stride[2])
+        if len(stride) == 3 and stride[2] == 1:
+            return lib.pack_rows(t.data_ptr(), 0, stride[0], stride[1])
     if not isinstance(t, torch.Tensor) or t.dim() not in (3, 4):
         raise ValueError("%s must be a [B,S,H,D] or [tokens,H,D] tensor" % name)
-    if not t.is_cuda or t.device != device:
-        raise ValueError("%s must be on device %s" % (name, device))
+    if t.get_device() != index:
+        raise ValueError("%s must be on device cuda:%d" % (name, index))
     if t.dtype != dtype:
         raise ValueError("%s must have dtype %s, not %s" % (name, dtype, t.dtype))
     if shape is not None and t.shape != shape:
         raise ValueError("%s must have shape %s, not %s" % (name, tuple(shape), tuple(t.shape)))
-    stride = t.stride()
-    if stride[-1] != 1:
-        raise ValueError("the last axis of %s must be contiguous" % name)
-    return lib.Rows(t.data_ptr(), stride[0] if len(stride) == 4 else 0, stride[-3], stride[-2])
+    raise ValueError("the last axis of %s must be contiguous" % name)
 
 
-def _call(fn, device, *args):
-    """Calls a C entry point on the current stream of `device`, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        st = fn(*args, lib.current_stream())
+def _plain(t, name, dtype, shape, index):
+    """Address of a contiguous tensor of this type and shape on device `index`."""
+    if not (isinstance(t, torch.Tensor) and t.dtype == dtype and t.get_device() == index and t.shape == shape
+            and t.is_contiguous()):
+        _check(t, name, dtype, shape, torch.device("cuda", index))
+    return t.data_ptr()
+
+
+def _call(fn, index, *args):
+    """Calls a C entry point on the current stream of device `index`, whichever device is current."""
+    if index == torch.cuda.current_device():
+        st = fn(*args, lib.raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            st = fn(*args, lib.current_stream())
+        with torch.cuda.device(index):
+            st = fn(*args, lib.raw_stream(index))
     if st:
         lib.check(st)
 
 
-def _workspace(workspace, need, device, name="workspace"):
+def _workspace(workspace, need, index):
+    """(address, bytes) of a workspace, and the tensor that holds it."""
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    if not (isinstance(workspace, torch.Tensor) and workspace.is_cuda and workspace.device == device
-            and workspace.is_contiguous()):
-        raise ValueError("%s must be a contiguous tensor on %s" % (name, device))
-    return workspace
+        if not need:
+            return None, 0, None
+        workspace = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", index))
+        return workspace.data_ptr(), need, workspace
+    if not (isinstance(workspace, torch.Tensor) and workspace.get_device() == index and workspace.is_contiguous()):
+        raise ValueError("workspace must be a contiguous tensor on cuda:%d" % index)
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
-def _bytes(t):
-    return t.numel() * t.element_size()
+_contiguous = torch.contiguous_format
 
 
 def _norm_rope_args(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved):
     if not isinstance(q, torch.Tensor) or q.dtype not in _DTYPES or not q.is_cuda or q.dim() not in (3, 4):
         raise ValueError("q must be a float32 or bfloat16 device tensor [B,S,H,D] or [tokens,H,D]")
-    device, dtype = q.device, q.dtype
-    rq, rk = _rows(q, "q", dtype, device), _rows(k, "k", dtype, device)
-    if k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+    index, dtype = q.get_device(), q.dtype
+    rq, rk = _rows(q, "q", dtype, index), _rows(k, "k", dtype, index)
+    shape, k_shape = q.shape, k.shape
+    Hq, D = shape[-2:]
+    if k_shape[:-2] != shape[:-2] or k_shape[-1] != D:
         raise ValueError("k must have q's tokens and head dimension")
-    D = q.shape[-1]
-    _check(q_weight, "q_weight", dtype, (D,), device)
-    _check(k_weight, "k_weight", dtype, (D,), device)
-    _check(positions, "positions", torch.int32, q.shape[:-2], device)
     if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1:
         raise ValueError("inv_freq must be a tensor of one frequency for each rotated pair")
-    _check(inv_freq, "inv_freq", torch.float32, inv_freq.shape, device)
-    B = q.shape[0] if q.dim() == 4 else 1
-    tail = (positions.data_ptr(), inv_freq.data_ptr(), _DTYPES[dtype], B, q.shape[-3], q.shape[-2], k.shape[-2], D,
-            2 * inv_freq.shape[0], int(bool(interleaved)), eps)
-    return rq, rk, tail
+    pairs = inv_freq.shape[0]
+    args = (_plain(q_weight, "q_weight", dtype, (D,), index), _plain(k_weight, "k_weight", dtype, (D,), index),
+            _plain(positions, "positions", torch.int32, shape[:-2], index),
+            _plain(inv_freq, "inv_freq", torch.float32, (pairs,), index), _DTYPES[dtype],
+            shape[0] if len(shape) == 4 else 1, shape[-3], Hq, k_shape[-2], D, 2 * pairs, 1 if interleaved else 0, eps)
+    return index, rq, rk, args
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interleaved=False, out=None):
@@ -254,15 +272,14 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interl
     are rotated: elements i and i + len, or 2i and 2i + 1 if `interleaved`).  Returns the new
     (q, k), written to the pair `out` if given; out=(q, k) works in place.  kcg_qk_norm_rope.
     """
-    rq, rk, tail = _norm_rope_args(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    index, rq, rk, args = _norm_rope_args(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
     if out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        q_out = torch.empty_like(q, memory_format=_contiguous)
+        k_out = torch.empty_like(k, memory_format=_contiguous)
     else:
         q_out, k_out = out
-    ro = _rows(q_out, "out[0]", q.dtype, q.device, q.shape)
-    rp = _rows(k_out, "out[1]", q.dtype, q.device, k.shape)
-    _call(lib.load().kcg_qk_norm_rope, q.device, rq, rk, ro, rp, q_weight.data_ptr(), k_weight.data_ptr(), *tail)
+    _call(lib.load().kcg_qk_norm_rope, index, rq, rk, _rows(q_out, "out[0]", q.dtype, index, q.shape),
+          _rows(k_out, "out[1]", q.dtype, index, k.shape), *args)
     return q_out, k_out
 
 
@@ -273,19 +290,16 @@ def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, positions, inv_freq,
     The other arguments are the forward call's inputs.  workspace: a contiguous device tensor
     of at least kcg_qk_norm_rope_backward_ws_bytes bytes (allocated if not given).
     """
-    rq, rk, tail = _norm_rope_args(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
-    rdq = _rows(dq, "dq", q.dtype, q.device, q.shape)
-    rdk = _rows(dk, "dk", q.dtype, q.device, k.shape)
+    index, rq, rk, args = _norm_rope_args(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
+    dtype, shape, k_shape = q.dtype, q.shape, k.shape
+    rdq, rdk = _rows(dq, "dq", dtype, index, shape), _rows(dk, "dk", dtype, index, k_shape)
     L = lib.load()
-    gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    gk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    gq, gk = torch.empty_like(q, memory_format=_contiguous), torch.empty_like(k, memory_format=_contiguous)
     gwq, gwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
-    rgq, rgk = _rows(gq, "grad_q", q.dtype, q.device), _rows(gk, "grad_k", q.dtype, q.device)
-    ws = _workspace(workspace, L.kcg_qk_norm_rope_backward_ws_bytes(*tail[3:8]), q.device)
-    if ws is None:  # a shape that the call itself refuses
-        ws = torch.empty(16, dtype=torch.uint8, device=q.device)
-    _call(L.kcg_qk_norm_rope_backward, q.device, rdq, rdk, rq, rk, rgq, rgk, q_weight.data_ptr(), k_weight.data_ptr(),
-          gwq.data_ptr(), gwk.data_ptr(), *tail, ws.data_ptr(), _bytes(ws))
+    # (a shape that has no workspace is one that the call refuses)
+    address, size, held = _workspace(workspace, L.kcg_qk_norm_rope_backward_ws_bytes(*args[5:10]) or 16, index)
+    _call(L.kcg_qk_norm_rope_backward, index, rdq, rdk, rq, rk, _rows(gq, "grad_q", dtype, index),
+          _rows(gk, "grad_k", dtype, index), args[0], args[1], gwq.data_ptr(), gwk.data_ptr(), *args[2:], address, size)
     return gq, gk, gwq, gwk
 
 
@@ -311,7 +325,7 @@ class KvCache:
         elif k_exp is not None or v_exp is not None:
             raise ValueError("a bfloat16 cache has no exponents")
         self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
-        self.device = k.device
+        self.index = k.get_device()
         pages, self.heads, self.page_size, self.dim = k.shape
         eight = k.dtype == torch.float8_e4m3fn
         if max(k.shape) > 0x7fffffff:
@@ -329,10 +343,10 @@ class KvCache:
         return cls(k, v, *(torch.empty((pages, heads, page_size), dtype=torch.uint8, device=device) for _ in range(2)))
 
 
-def _cache_check(cache):
+def _cache_device(cache):
     if not isinstance(cache, KvCache):
         raise ValueError("cache must be a KvCache")
-    return cache.device
+    return cache.index
 
 
 def kv_cache_write(cache, k, v, slots):
@@ -342,16 +356,15 @@ def kv_cache_write(cache, k, v, slots):
     not written, and of tokens with the same slot the last one is.  fp32 or bf16 rows are
     rounded to the cache's type; kcg_kv_cache_write says how.
     """
-    device = _cache_check(cache)
+    index = _cache_device(cache)
     if not isinstance(k, torch.Tensor) or k.dtype not in _DTYPES:
         raise ValueError("k must be a float32 or bfloat16 tensor")
-    rk = _rows(k, "k", k.dtype, device)
-    rv = _rows(v, "v", k.dtype, device, k.shape)
-    if k.shape[-2:] != (cache.heads, cache.dim):
+    dtype, shape = k.dtype, k.shape
+    rk, rv = _rows(k, "k", dtype, index), _rows(v, "v", dtype, index, shape)
+    if shape[-2:] != (cache.heads, cache.dim):
         raise ValueError("k must have the cache's heads and dim %s" % ((cache.heads, cache.dim),))
-    _check(slots, "slots", torch.int32, k.shape[:-2], device)
-    B = k.shape[0] if k.dim() == 4 else 1
-    _call(lib.load().kcg_kv_cache_write, device, cache._c, rk, rv, _DTYPES[k.dtype], slots.data_ptr(), B, k.shape[-3])
+    _call(lib.load().kcg_kv_cache_write, index, cache._c, rk, rv, _DTYPES[dtype],
+          _plain(slots, "slots", torch.int32, shape[:-2], index), shape[0] if len(shape) == 4 else 1, shape[-3])
 
 
 def kv_cache_read(cache, slots, out_dtype=torch.bfloat16, out=None):
@@ -360,28 +373,31 @@ def kv_cache_read(cache, slots, out_dtype=torch.bfloat16, out=None):
     A slot outside the cache gives rows of zeros.  out: the pair of tensors to write, with any
     strides but a contiguous last axis.
     """
-    device = _cache_check(cache)
+    index = _cache_device(cache)
     if not isinstance(slots, torch.Tensor) or slots.dim() not in (1, 2):
         raise ValueError("slots must be an int32 tensor [B,S] or [tokens]")
-    _check(slots, "slots", torch.int32, slots.shape, device)
-    shape = torch.Size(tuple(slots.shape) + (cache.heads, cache.dim))
+    shape = tuple(slots.shape)
+    at = _plain(slots, "slots", torch.int32, shape, index)
+    B, S = shape if len(shape) == 2 else (1, shape[0])
+    shape += (cache.heads, cache.dim)
     if out is None:
-        k = torch.empty(shape, dtype=out_dtype, device=device)
-        v = torch.empty(shape, dtype=out_dtype, device=device)
+        if out_dtype not in _DTYPES:
+            raise ValueError("a cache is read as float32 or bfloat16")
+        k = torch.empty(shape, dtype=out_dtype, device=cache.k.device)
+        v = torch.empty_like(k)
     else:
         k, v = out
-    dtype = k.dtype if isinstance(k, torch.Tensor) else None
-    if dtype not in _DTYPES:
-        raise ValueError("a cache is read as float32 or bfloat16")
-    rk, rv = _rows(k, "out[0]", dtype, device, shape), _rows(v, "out[1]", dtype, device, shape)
-    B = slots.shape[0] if slots.dim() == 2 else 1
-    _call(lib.load().kcg_kv_cache_read, device, cache._c, slots.data_ptr(), rk, rv, _DTYPES[dtype], B, slots.shape[-1])
+        out_dtype = k.dtype if isinstance(k, torch.Tensor) else None
+        if out_dtype not in _DTYPES:
+            raise ValueError("a cache is read as float32 or bfloat16")
+    _call(lib.load().kcg_kv_cache_read, index, cache._c, at, _rows(k, "out[0]", out_dtype, index, shape),
+          _rows(v, "out[1]", out_dtype, index, shape), _DTYPES[out_dtype], B, S)
     return k, v
 
 
 def fmha_cache_workspace_bytes(cache, table_width, batch, drafts, heads):
     """Bytes of workspace with which fmha_cache can split long sequences as it prefers to."""
-    _cache_check(cache)
+    _cache_device(cache)
     return int(lib.load().kcg_fmha_cache_ws_bytes(cache._c, table_width, batch, drafts, heads))
 
 
@@ -395,37 +411,32 @@ def fmha_cache(q, cache, block_table, context_lens, draft_lens=None, tree_mask=N
     that drafted token n sees drafted token j (default: a chain, j <= n).  Lengths and table are
     int32.  Rows of `out` from draft_lens[b] on stay as they were.  kcg_fmha_cache says the rest.
     """
-    device = _cache_check(cache)
+    index = _cache_device(cache)
     if not isinstance(q, torch.Tensor) or q.dim() != 4:
         raise ValueError("q must be a [B,N,H,dim] tensor")
-    rq = _rows(q, "q", torch.bfloat16, device)
-    B, N, Hq, D = q.shape
+    rq = _rows(q, "q", torch.bfloat16, index)
+    shape = q.shape
+    B, N, Hq, D = shape
     if D != cache.dim or Hq % cache.heads:
         raise ValueError("q must have the cache's dim and a multiple of its heads")
     if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
         raise ValueError("block_table must be an int32 tensor [B, pages]")
     width = block_table.shape[1]
-    _check(block_table, "block_table", torch.int32, (B, width), device)
-    _check(context_lens, "context_lens", torch.int32, (B,), device)
-    if draft_lens is not None:
-        _check(draft_lens, "draft_lens", torch.int32, (B,), device)
-    if tree_mask is not None:
-        _check(tree_mask, "tree_mask", torch.int64, (B, N), device)
+    table = _plain(block_table, "block_table", torch.int32, (B, width), index)
+    context = _plain(context_lens, "context_lens", torch.int32, (B,), index)
+    drafts = None if draft_lens is None else _plain(draft_lens, "draft_lens", torch.int32, (B,), index)
+    tree = None if tree_mask is None else _plain(tree_mask, "tree_mask", torch.int64, (B, N), index)
     if out is None:
-        if draft_lens is not None:
-            out = torch.zeros(q.shape, dtype=out_dtype or torch.bfloat16, device=device)
-        else:
-            out = torch.empty(q.shape, dtype=out_dtype or torch.bfloat16, device=device)
-    elif out_dtype not in (None, out.dtype):
-        raise ValueError("out must have dtype %s, not %s" % (out_dtype, out.dtype))
-    if out.dtype not in _DTYPES:
-        raise ValueError("attention over a cache writes bfloat16 or float32, not %s" % out.dtype)
-    ro = _rows(out, "out", out.dtype, device, q.shape)
+        out_dtype = out_dtype or torch.bfloat16
+        out = (torch.empty if draft_lens is None else torch.zeros)(shape, dtype=out_dtype, device=q.device)
+    elif not isinstance(out, torch.Tensor) or out_dtype not in (None, out.dtype):
+        raise ValueError("out must be a tensor of dtype out_dtype")
+    out_dtype = out.dtype
+    if out_dtype not in _DTYPES:
+        raise ValueError("attention over a cache writes bfloat16 or float32, not %s" % out_dtype)
     L = lib.load()
-    need = L.kcg_fmha_cache_ws_bytes(cache._c, width, B, N, Hq)
-    ws = _workspace(workspace, need, device)
-    _call(L.kcg_fmha_cache, device, rq, cache._c, block_table.data_ptr(), width, context_lens.data_ptr(),
-          draft_lens.data_ptr() if draft_lens is not None else None,
-          tree_mask.data_ptr() if tree_mask is not None else None, ro, _DTYPES[out.dtype], B, N, Hq, scale,
-          ws.data_ptr() if ws is not None else None, _bytes(ws) if ws is not None else 0)
+    address, size, held = _workspace(workspace, workspace is None and L.kcg_fmha_cache_ws_bytes(cache._c, width, B, N, Hq),
+                                     index)
+    _call(L.kcg_fmha_cache, index, rq, cache._c, table, width, context, drafts, tree,
+          _rows(out, "out", out_dtype, index, shape), _DTYPES[out_dtype], B, N, Hq, scale, address, size)
     return out

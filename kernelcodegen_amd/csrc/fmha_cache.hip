@@ -50,7 +50,8 @@ struct FmhaCacheArgs {
   float *partial;  // [unit][head][tile][rows][D], then the logarithms [unit][head][tile][rows]
   int64_t logs;    // where those begin, in floats
   int B, N, Hq, width, group, tiles, rows, want_units, max_units;
-  float q_sign, c;
+  float c;
+  unsigned q_flip;  // sign bits of two bf16 numbers, or 0
   bool vec;
 };
 
@@ -67,9 +68,14 @@ __device__ __forceinline__ KvLens fc_lens(const FmhaCacheArgs<C> &a, int b) {
                  static_cast<int64_t>(a.width) << a.cache.shape.log2_page);
 }
 
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m);
+// Sum over the lanes up to and with this one, in registers (row shifts, then the rows' last lanes handed on).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
   return x;
 }
 
@@ -84,7 +90,7 @@ __device__ __forceinline__ bool find_unit(const FmhaCacheArgs<C> &a, int unit, F
     l = {0, 0, 0};
     if (b0 + lane < a.B) l = fc_lens(a, b0 + lane);
     const int chunks = l.queries ? (l.context + l.drafts + kFcChunk - 1) / kFcChunk : 0;
-    total += __builtin_amdgcn_readfirstlane(wave_sum(chunks));
+    total += __builtin_amdgcn_readlane(wave_scan(chunks), 63);
   }
   int64_t per = (total + a.want_units - 1) / a.want_units;
   per = per < kFcMinChunks ? kFcMinChunks : per > (1 << 30) ? 1 << 30 : per;  // (no sequence has as many)
@@ -97,12 +103,7 @@ __device__ __forceinline__ bool find_unit(const FmhaCacheArgs<C> &a, int unit, F
     }
     const int chunks = (l.context + l.drafts + kFcChunk - 1) / kFcChunk;
     const int units = !l.queries ? 0 : chunks <= per ? 1 : (chunks + static_cast<int>(per) - 1) / static_cast<int>(per);
-    int upto = units;
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-      const int other = __shfl_up(upto, m);
-      if (lane >= m) upto += other;
-    }
+    const int upto = wave_scan(units);
     const bool mine = unit >= 0 ? units && unit >= before + upto - units && unit < before + upto : b0 + lane == -1 - unit;
     const uint64_t found = __ballot(mine);
     if (found) {
@@ -235,15 +236,7 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
 
   uint8_t *ring = lds + wave * 2 * T::kBuffer;
   const unsigned ring_at = __builtin_amdgcn_readfirstlane(lds_address(ring));
-  // byte offsets of this lane's pieces from the first row of a load
-  const int load_row = lane / T::kPieces, load_pos = lane % T::kPieces;
-  unsigned off_k[T::kLoads], off_v[T::kLoads];
-#pragma unroll
-  for (int j = 0; j < T::kLoads; ++j) {
-    const int row = j * T::kRowsPerLoad + load_row;
-    off_k[j] = load_row * T::kRow + (load_pos ^ T::swizzle_k(row)) * 16;
-    off_v[j] = load_row * T::kRow + (load_pos ^ T::swizzle_v(row)) * 16;
-  }
+  const int load_row = lane / T::kPieces;
   int valid[2] = {0, 0};  // per buffer: bit g: the page of keys 16 g .. 16 g + 15 is the cache's
   auto load_chunk = [&](int chunk, int buffer) {
     const int key0 = chunk * kFcChunk;
@@ -257,12 +250,17 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
     const unsigned to = ring_at + buffer * T::kBuffer;
     // the buffer's last reads are done (their results are used), as far as the hardware is told
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // byte offsets of this lane's pieces from the first row of a load; computed for each chunk, since
+    // registers are scarcer than these few instructions
+    int l_row = load_row, l_pos = lane % T::kPieces;
+    asm volatile("" : "+v"(l_row), "+v"(l_pos));
 #pragma unroll
     for (int j = 0; j < T::kLoads; ++j) {
       const int first = j * T::kRowsPerLoad;
       const int64_t row = base[first / 16] + first % 16;
-      direct_load_16B(a.cache.k + row * D, off_k[j], to + j * 1024);
-      direct_load_16B(a.cache.v + row * D, off_v[j], to + T::kBytes + j * 1024);
+      direct_load_16B(a.cache.k + row * D, l_row * T::kRow + (l_pos ^ T::swizzle_k(first + l_row)) * 16, to + j * 1024);
+      direct_load_16B(a.cache.v + row * D, l_row * T::kRow + (l_pos ^ T::swizzle_v(first + l_row)) * 16,
+                      to + T::kBytes + j * 1024);
     }
     if constexpr (E8) {
       // dwords 0-7: K's exponents, 8-15: V's (the other lanes repeat them)
@@ -277,30 +275,33 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
 
   // ---- Q ----
   // The last QL steps of Q are kept in LDS where the accumulators of two tiles leave no registers for them.
-  constexpr int QL = D * QT == 256 && E8 && TERMS == 1 ? 4 : 0;
+  constexpr int QL = D * QT == 256 && E8 && TERMS == 1 ? 5 : 0;
   __shared__ uint4_t q_lds[QL ? QT : 1][QL ? QL : 1][QL ? 64 : 1];
   bf16x8_v q[QT][DS - QL];
-  uint64_t seen[QT];
+  // Columns beyond the last row repeat it: what they compute is never stored.
+  const int last_row = u.len.queries * a.group - 1;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    const int row = row0 + 32 * t + r32;
+    const int row = min(row0 + 32 * t + r32, last_row);
     const int node = row / a.group, h = head * a.group + row - node * a.group;
-    const bool live = node < u.len.queries;
-    seen[t] = live ? kv_seen(a.tree, static_cast<int64_t>(b) * a.N + node, node, u.len.drafts) : 0;
+    const uint16_t *from = a.q.at(b, node, h) + (E8 ? 16 : 8) * half;
+    auto d_of = [](int s) { return E8 ? 32 * (s / 2) + 8 * (s % 2) : 16 * s; };
+    uint4_t x[DS];
+    if (a.vec) {
+#pragma unroll
+      for (int s = 0; s < DS; ++s) x[s] = *reinterpret_cast<const uint4_t *>(from + d_of(s));
+    } else {
+#pragma unroll
+      for (int s = 0; s < DS; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[s][j] = from[d_of(s) + 2 * j] | static_cast<unsigned>(from[d_of(s) + 2 * j + 1]) << 16;
+    }
 #pragma unroll
     for (int s = 0; s < DS; ++s) {
-      float x[8] = {};
-      const int d = E8 ? 32 * (s / 2) + 16 * half + 8 * (s % 2) : 16 * s + 8 * half;
-      if (live) {
-        const uint16_t *from = a.q.at(b, node, h) + d;
-        if (a.vec) load8<true>(from, x);
-        else load8<false>(from, x);
-      }
-      bf16x8_v y;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = static_cast<__bf16>(x[j] * a.q_sign);
-      if (s < DS - QL) q[t][s] = y;
-      else if (wave == s - (DS - QL)) q_lds[QL ? t : 0][QL ? s - (DS - QL) : 0][QL ? lane : 0] = __builtin_bit_cast(uint4_t, y);
+      for (int j = 0; j < 4; ++j) x[s][j] ^= a.q_flip;
+      if (s < DS - QL) q[t][s] = __builtin_bit_cast(bf16x8_v, x[s]);
+      else if (wave == (s - (DS - QL)) % kFcWaves) q_lds[QL ? t : 0][QL ? s - (DS - QL) : 0][QL ? lane : 0] = x[s];
     }
   }
   if (QL) __syncthreads();
@@ -321,12 +322,6 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
       for (int e = 0; e < 16; ++e) acc[t][i][e] = 0.0f;
   }
 
-  // V: row and byte column of this lane's transposing reads, within 16 keys and 32 columns
-  const int l16 = lane & 15, side = (lane >> 4) & 1;
-  const int v_row = E8 ? 4 * half + ((l16 >> 1) & 3) + 8 * (l16 >> 3) : 4 * half + (l16 >> 2);
-  const int v_piece = E8 ? side : 2 * side + ((l16 & 3) >> 1);
-  const int v_at = v_row * T::kRow + (l16 & 1) * 8;
-
   for (int chunk = begin; chunk < end; ++chunk) {
     const int buffer = (chunk - begin) & 1;
     if (chunk + 1 < end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::kLoadsPerChunk) : "memory");
@@ -334,6 +329,15 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
     const uint8_t *ks = ring + buffer * T::kBuffer;
     uint8_t *vs = ring + buffer * T::kBuffer + T::kBytes;
     const uint8_t *xs = vs + T::kBytes;
+    // The lane's addresses; where registers are scarce they are computed for each chunk.
+    int at = lane;
+    if (QL) asm volatile("" : "+v"(at));
+    const int k_row = at & 31, k_half = at >> 5;
+    // V: row and byte column of this lane's transposing reads, within 16 keys and 32 columns
+    const int l16 = at & 15, side = (at >> 4) & 1;
+    const int v_row = E8 ? 4 * k_half + ((l16 >> 1) & 3) + 8 * (l16 >> 3) : 4 * k_half + (l16 >> 2);
+    const int v_piece = E8 ? side : 2 * side + ((l16 & 3) >> 1);
+    const int v_at = v_row * T::kRow + (l16 & 1) * 8;
 
     // ---- S^T = K . Q^T ----
     float16_t s[QT];
@@ -342,10 +346,10 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
     if constexpr (E8) {
-      const float scale = exponent_to_scale(xs[r32]);
+      const float scale = exponent_to_scale(xs[k_row]);
 #pragma unroll
       for (int p = 0; p < D / 32; ++p) {
-        const uint4_t x = *reinterpret_cast<const uint4_t *>(ks + r32 * T::kRow + ((2 * p + half) ^ T::swizzle_k(r32)) * 16);
+        const uint4_t x = *reinterpret_cast<const uint4_t *>(ks + k_row * T::kRow + ((2 * p + k_half) ^ T::swizzle_k(k_row)) * 16);
         const bf16x8_v k0 = to_bf16(x[0], x[1], scale), k1 = to_bf16(x[2], x[3], scale);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
@@ -356,7 +360,7 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
     } else {
 #pragma unroll
       for (int p = 0; p < DS; ++p) {
-        const uint4_t x = *reinterpret_cast<const uint4_t *>(ks + r32 * T::kRow + ((2 * p + half) ^ T::swizzle_k(r32)) * 16);
+        const uint4_t x = *reinterpret_cast<const uint4_t *>(ks + k_row * T::kRow + ((2 * p + k_half) ^ T::swizzle_k(k_row)) * 16);
         const bf16x8_v k = __builtin_bit_cast(bf16x8_v, x);
 #pragma unroll
         for (int t = 0; t < QT; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q_of(t, p), s[t], 0, 0, 0);
@@ -372,9 +376,11 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
       unsigned vis[QT];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
+        const int node = min(row0 + 32 * t + r32, last_row) / a.group;
+        const uint64_t seen = kv_seen(a.tree, static_cast<int64_t>(b) * a.N + node, node, u.len.drafts);
         unsigned v;
-        if (d0 >= 0) v = d0 < 64 ? static_cast<unsigned>(seen[t] >> d0) : 0u;
-        else if (d0 > -32) v = static_cast<unsigned>(seen[t] << -d0) | ((1u << -d0) - 1);
+        if (d0 >= 0) v = d0 < 64 ? static_cast<unsigned>(seen >> d0) : 0u;
+        else if (d0 > -32) v = static_cast<unsigned>(seen << -d0) | ((1u << -d0) - 1);
         else v = 0xffffffffu;
         vis[t] = v & there;
         const unsigned mine = vis[t] >> (4 * half);
@@ -433,6 +439,35 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
       }
     }
 
+    // ---- V^T of the first 16 keys, before the weights are computed: an LDS read takes longer than the
+    // products between two ----
+    constexpr int kWords = E8 ? 2 : 4;
+    unsigned v_raw[2][DT][kWords];
+    auto read_v = [&](int kb) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i) {
+        // rows 16 apart have one swizzle, and with b16 reads rows 8 apart
+        const int piece = ((E8 ? 2 : 4) * i + v_piece) ^ T::swizzle_v(v_row);
+        const uint8_t *from = vs + kb * 16 * T::kRow + v_at + piece * 16;
+        if constexpr (E8) {
+          const int2_v x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_v *)from);
+          v_raw[kb][i][0] = static_cast<unsigned>(x[0]);
+          v_raw[kb][i][1] = static_cast<unsigned>(x[1]);
+        } else {
+          const uint2_t lo = __builtin_bit_cast(
+              uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4_v *)from));
+          const uint2_t hi = __builtin_bit_cast(
+              uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4_v *)(from + 8 * T::kRow)));
+          v_raw[kb][i][0] = lo[0];
+          v_raw[kb][i][1] = lo[1];
+          v_raw[kb][i][2] = hi[0];
+          v_raw[kb][i][3] = hi[1];
+        }
+      }
+      asm volatile("" ::: "memory");  // (or the compiler moves the reads down to their uses)
+    };
+    read_v(0);
+
     // ---- weights ----
     unsigned p[QT][TERMS][8];  // bf16 pairs: elements 2w, 2w + 1
 #pragma unroll
@@ -458,7 +493,7 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
       if constexpr (E8) {
 #pragma unroll
         for (int g = 0; g < 4; ++g)  // V's exponents of the keys 8 g + 4 half .. + 3, less 128
-          x[g] = *reinterpret_cast<const unsigned *>(xs + 32 + 8 * g + 4 * half) ^ 0x80808080u;
+          x[g] = *reinterpret_cast<const unsigned *>(xs + 32 + 8 * g + 4 * k_half) ^ 0x80808080u;
       }
 #pragma unroll
       for (int w2 = 0; w2 < 8; ++w2) {
@@ -491,24 +526,14 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
     }
 
     // ---- O^T += V^T . P^T ----
+    read_v(1);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int i = 0; i < DT; ++i) {
         bf16x8_v v;
-        if constexpr (E8) {
-          const int piece = (2 * i + v_piece) ^ T::swizzle_v(v_row);  // rows 16 apart have one swizzle
-          const int2_v x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-              (__attribute__((address_space(3))) int2_v *)(vs + kb * 16 * T::kRow + v_at + piece * 16));
-          v = to_bf16(static_cast<unsigned>(x[0]), static_cast<unsigned>(x[1]), 1.0f);
-        } else {
-          const int piece = (4 * i + v_piece) ^ T::swizzle_v(v_row);  // rows 8 and 16 apart have one swizzle
-          const uint8_t *from = vs + kb * 16 * T::kRow + v_at + piece * 16;
-          const bf16x4_v lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4_v *)from);
-          const bf16x4_v hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-              (__attribute__((address_space(3))) bf16x4_v *)(from + 8 * T::kRow));
-          v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
+        if constexpr (E8) v = to_bf16(v_raw[kb][i][0], v_raw[kb][i][1], 1.0f);
+        else v = __builtin_bit_cast(bf16x8_v, uint4_t{v_raw[kb][i][0], v_raw[kb][i][1], v_raw[kb][i][2], v_raw[kb][i][3]});
 #pragma unroll
         for (int t = 0; t < QT; ++t)
 #pragma unroll
@@ -640,6 +665,7 @@ __global__ __launch_bounds__(256) void fmha_cache_join_kernel(const FmhaCacheArg
 // How a call is split; the query and the call agree on it.
 struct FcPlan {
   int group, rows_all, qt, tiles, rows;  // rows: of a tile that are stored
+  int places;                            // workgroups that a CU holds
   int want_units, max_units;
   int64_t floats;  // workspace
 };
@@ -651,9 +677,15 @@ inline FcPlan plan_fmha_cache(const kcg_kv_cache &c, int width, int B, int N, in
   p.qt = p.rows_all <= 32 ? 1 : 2;
   p.tiles = (p.rows_all + 32 * p.qt - 1) / (32 * p.qt);
   p.rows = p.tiles > 1 ? 64 : p.rows_all;
+  p.places = c.dtype == KCG_E4M3 || c.dim == 64 ? 2 : 1;  // (a bf16 ring of 128 elements is 128 KiB)
   const int64_t per_unit = static_cast<int64_t>(c.heads) * p.tiles;
-  // units so that there are some workgroups to each of the CU's two places
-  int64_t want = (2048 + per_unit - 1) / per_unit;
+  const int64_t round = 256 * p.places / per_unit;  // units that run at once
+  // A few sequences: one round, less the unit that each sequence's remainder may add (a tree of 32 over 131072
+  // keys: 119 us, 130 with two rounds, 168 with four).  Many: rounds enough that the last one, which
+  // is not full, does not count for much (64 single tokens over contexts to 8192: 131 us with one, 120
+  // with 1.25 to 2.75, 124 with four).
+  int64_t want = 8 * B <= round ? round - B : 5 * round / 2;
+  if (want < 1) want = 1;
   const int64_t chunks = (static_cast<int64_t>(width) * c.page_size + kFcChunk - 1) / kFcChunk;
   const int64_t most = B * ((chunks + kFcMinChunks - 1) / kFcMinChunks);
   if (want > most) want = most;
@@ -713,9 +745,10 @@ int fmha_cache(const kcg_rows &q, const kcg_kv_cache &cache, const int32_t *tabl
   a.rows = p.rows;
   a.want_units = split ? p.want_units : 1;
   a.max_units = p.max_units;
-  // the scale's sign goes into Q, so that the maximum of the scores is that of the products
-  a.q_sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;
-  a.c = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504088896340736f;
+  // The scale's sign goes into Q, so that the maximum of the scores is that of the products.  For a scale
+  // of 0 the smallest normal number stands: its products vanish beside 1, and -inf stays -inf under it.
+  a.q_flip = scale < 0.0f ? 0x80008000u : 0u;
+  a.c = scale == 0.0f ? 1.17549435e-38f : fabsf(scale) * 1.44269504088896340736f;
   a.vec = rows_aligned16(q, KCG_BF16, B, N, Hq) && rows_aligned16(out, o_dtype, B, N, Hq);
 #define KCG_PICK(DD, QQ) \
   return o_dtype == KCG_F32 ? run_fmha_cache<C, DD, QQ, 3>(a, split, stream) : run_fmha_cache<C, DD, QQ, 1>(a, split, stream)

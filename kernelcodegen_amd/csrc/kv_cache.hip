@@ -15,45 +15,51 @@ struct KvMoveArgs {
   KvCache<C> cache;
   const int32_t *slots;
   int S, tokens;
+  int first, end;  // writing: the tokens of this launch
 };
 
-// The least x in [1, 254] with amax <= 448 * 2^(x - 127), for a finite amax: 448 is 1.75 * 2^8.
-__device__ __forceinline__ int e4m3_exponent(float amax) {
-  const unsigned bits = __builtin_bit_cast(unsigned, amax);
+// The least x in [1, 254] with amax <= 448 * 2^(x - 127), from the bits of a finite amax: 448 is 1.75 * 2^8.
+__device__ __forceinline__ int e4m3_exponent(unsigned bits) {
   const int x = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
   return x < 1 ? 1 : x;
 }
 
+constexpr unsigned kInfBits = 0x7f800000u;
+
+__device__ __forceinline__ unsigned magnitude_bits(float x) { return __builtin_bit_cast(unsigned, x) & 0x7fffffffu; }
+
 // Eight elements of a row into the cache.
 template <int LANES>
-__device__ __forceinline__ void cache_store8(uint16_t *to, uint8_t *, const float (&x)[8], int) {
+__device__ __forceinline__ void cache_store8(uint16_t *to, uint8_t *, float (&x)[8], int) {
   store8<true>(to, x);
 }
 template <int LANES>
-__device__ __forceinline__ void cache_store8(uint8_t *to, uint8_t *exponent, const float (&x)[8], int lane_in_row) {
-  float amax = 0.0f;
+__device__ __forceinline__ void cache_store8(uint8_t *to, uint8_t *exponent, float (&x)[8], int lane_in_row) {
+  // magnitudes compare as their bits do; infinity and NaN are the largest
+  unsigned top = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float m = fabsf(x[j]);
-    amax = m < INFINITY ? fmaxf(amax, m) : amax;
+  for (int j = 0; j < 8; ++j) top = max(top, magnitude_bits(x[j]));
+  top = row_max<LANES>(top);
+  unsigned nan[2] = {0, 0};
+  if (top >= kInfBits) {  // rare: the row's largest finite magnitude, and which elements become NaN
+    top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool finite = magnitude_bits(x[j]) < kInfBits;
+      if (finite) top = max(top, magnitude_bits(x[j]));
+      else nan[j / 4] |= 0x7fu << (8 * (j % 4));
+      x[j] = finite ? x[j] : 0.0f;
+    }
+    top = row_max<LANES>(top);
   }
-  amax = row_max<LANES>(amax);
-  const int e = e4m3_exponent(amax);
+  const int e = e4m3_exponent(top);
   const float inverse = exponent_to_scale(254 - e);
   uint2_t q;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    float y[4];
-    unsigned nan = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool finite = fabsf(x[4 * w + j]) < INFINITY;
-      y[j] = finite ? x[4 * w + j] * inverse : 0.0f;
-      nan |= finite ? 0u : 0x7fu << (8 * j);
-    }
-    int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-    p = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], p, true);
-    q[w] = static_cast<unsigned>(p) | nan;
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w] * inverse, x[4 * w + 1] * inverse, 0, false);
+    p = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w + 2] * inverse, x[4 * w + 3] * inverse, p, true);
+    q[w] = static_cast<unsigned>(p) | nan[w];
   }
   *reinterpret_cast<uint2_t *>(to) = q;
   if (lane_in_row == 0) *exponent = static_cast<uint8_t>(e);
@@ -62,74 +68,138 @@ __device__ __forceinline__ void cache_store8(uint8_t *to, uint8_t *exponent, con
 // GROUP tokens to a workgroup, all their heads.  A token that names the same slot as a later one is
 // left out, so that the last one is what the slot holds, whichever workgroup runs first: the
 // workgroup compares its GROUP slots with all that follow.  That is 4 bytes read per following
-// token and workgroup (tokens^2 / GROUP * 2 bytes from L2).
+// token and workgroup (2 tokens^2 / GROUP bytes, from L2); the first rows are on their way meanwhile.
 template <typename T, typename C, int D, bool VEC, int GROUP>
 __global__ __launch_bounds__(256) void kv_cache_write_kernel(const KvMoveArgs<const T, C> a) {
   constexpr int LANES = D / 8, PER = 256 / LANES;
   __shared__ int later[GROUP];
-  const int t0 = blockIdx.x * GROUP;
+  const int t0 = a.first + blockIdx.x * GROUP, end = a.end;
+  const int lane = threadIdx.x % LANES;
+  const int heads = a.cache.shape.heads, rows = 2 * heads;  // of a token: keys, then values
+  const int count = min(GROUP, end - t0);
+  // this lane's rows: PER apart in the order (token, row)
+  const int step_g = PER / rows, step_r = PER - step_g * rows;
+  int g = threadIdx.x / LANES / rows, r = threadIdx.x / LANES - g * rows;
+  auto load = [&](int g, int r, float(&x)[8]) {
+    const int t = t0 + g, b = a.S == a.tokens ? 0 : t / a.S, s = t - b * a.S;
+    load8<VEC>((r >= heads ? a.v.at(b, s, r - heads) : a.k.at(b, s, r)) + 8 * lane, x);
+  };
+  float x[8];
+  if (g < count) load(g, r, x);
   int slot[GROUP];
 #pragma unroll
-  for (int g = 0; g < GROUP; ++g) slot[g] = t0 + g < a.tokens ? a.slots[t0 + g] : -1;
+  for (int g = 0; g < GROUP; ++g) slot[g] = t0 + g < end ? a.slots[t0 + g] : -1;
   if (threadIdx.x < GROUP) later[threadIdx.x] = 0;
   __syncthreads();
-  for (int t = t0 + 1 + threadIdx.x; t < a.tokens; t += 256) {
-    const int s = a.slots[t];
+  auto compare = [&](int t, int s) {
+    unsigned least = 0xffffffffu;  // 0 if s is one of the slots
 #pragma unroll
-    for (int g = 0; g < GROUP; ++g)
-      if (s == slot[g] && t > t0 + g) later[g] = 1;
+    for (int g = 0; g < GROUP; ++g) least = min(least, static_cast<unsigned>(s ^ slot[g]));
+    if (least == 0) {
+#pragma unroll
+      for (int g = 0; g < GROUP; ++g)
+        if (s == slot[g] && t > t0 + g) later[g] = 1;
+    }
+  };
+  int t = t0 + 1 + threadIdx.x;
+  for (; t + 7 * 256 < end; t += 8 * 256) {  // eight loads under way
+    int s[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[k] = a.slots[t + 256 * k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) compare(t + 256 * k, s[k]);
   }
+  for (; t < end; t += 256) compare(t, a.slots[t]);
   __syncthreads();
-  const int lane = threadIdx.x % LANES;
-  const int rows = 2 * a.cache.shape.heads;  // of a token: keys, then values
-  for (int i = threadIdx.x / LANES; i < GROUP * rows; i += PER) {
-    const int g = i / rows, r = i - g * rows;
-    const bool is_v = r >= a.cache.shape.heads;
-    const int h = is_v ? r - a.cache.shape.heads : r;
-    const int t = t0 + g;
-    if (t >= a.tokens || later[g]) continue;
-    const int64_t row = kv_slot_row(a.cache.shape, a.slots[t], h);
-    if (row < 0) continue;
-    const int b = t / a.S, s = t - b * a.S;
-    float x[8];
-    load8<VEC>((is_v ? a.v.at(b, s, h) : a.k.at(b, s, h)) + 8 * lane, x);
-    cache_store8<LANES>((is_v ? a.cache.v : a.cache.k) + row * D + 8 * lane,
-                        (is_v ? a.cache.v_exp : a.cache.k_exp) + row, x, lane);
+  while (g < count) {
+    int next_g = g + step_g, next_r = r + step_r;
+    if (next_r >= rows) {
+      next_r -= rows;
+      ++next_g;
+    }
+    float next[8];
+    if (next_g < count) load(next_g, next_r, next);
+    const bool is_v = r >= heads;
+    const int64_t row = later[g] ? -1 : kv_slot_row(a.cache.shape, a.slots[t0 + g], is_v ? r - heads : r);
+    if (row >= 0)
+      cache_store8<LANES>((is_v ? a.cache.v : a.cache.k) + row * D + 8 * lane,
+                          (is_v ? a.cache.v_exp : a.cache.k_exp) + row, x, lane);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = next[j];
+    g = next_g;
+    r = next_r;
   }
 }
 
-template <typename T, typename C, int D, bool VEC>
-__global__ __launch_bounds__(256) void kv_cache_read_kernel(const KvMoveArgs<T, C> a) {
+// `group` tokens to a workgroup; up to ROWS rows of a lane are on their way at a time.
+template <typename T, typename C, int D, bool VEC, int ROWS>
+__global__ __launch_bounds__(256) void kv_cache_read_kernel(const KvMoveArgs<T, C> a, int group) {
   constexpr int LANES = D / 8, PER = 256 / LANES;
   const int lane = threadIdx.x % LANES;
-  const int rows = 2 * a.cache.shape.heads;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * PER + threadIdx.x / LANES;
-  const int t = static_cast<int>(i / rows), r = static_cast<int>(i - static_cast<int64_t>(t) * rows);
-  if (t >= a.tokens) return;
-  const bool is_v = r >= a.cache.shape.heads;
-  const int h = is_v ? r - a.cache.shape.heads : r;
-  const int64_t row = kv_slot_row(a.cache.shape, a.slots[t], h);
-  float x[8] = {};
-  if (row >= 0)
-    cache_load8((is_v ? a.cache.v : a.cache.k) + row * D + 8 * lane, (is_v ? a.cache.v_exp : a.cache.k_exp) + row, x);
-  const int b = t / a.S, s = t - b * a.S;
-  store8<VEC>((is_v ? a.v.at(b, s, h) : a.k.at(b, s, h)) + 8 * lane, x);
+  const int heads = a.cache.shape.heads, rows = 2 * heads;
+  const int t0 = blockIdx.x * group, count = min(group, a.tokens - t0);
+  const int step_g = PER / rows, step_r = PER - step_g * rows;
+  int g = threadIdx.x / LANES / rows, r = threadIdx.x / LANES - g * rows;
+  while (g < count) {
+    float x[ROWS][8];
+    T *to[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      to[k] = nullptr;
+      if (g < count) {
+        const int t = t0 + g, b = a.S == a.tokens ? 0 : t / a.S, s = t - b * a.S;
+        const bool is_v = r >= heads;
+        const int h = is_v ? r - heads : r;
+        to[k] = (is_v ? a.v.at(b, s, h) : a.k.at(b, s, h)) + 8 * lane;
+        const int64_t row = kv_slot_row(a.cache.shape, a.slots[t], h);
+        if (row >= 0) {
+          cache_load8((is_v ? a.cache.v : a.cache.k) + row * D + 8 * lane, (is_v ? a.cache.v_exp : a.cache.k_exp) + row,
+                      x[k]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[k][j] = 0.0f;
+        }
+      }
+      g += step_g;
+      r += step_r;
+      if (r >= rows) {
+        r -= rows;
+        ++g;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k)
+      if (to[k]) store8<VEC, true>(to[k], x[k]);
+  }
 }
 
 template <typename T, typename C, int D, bool VEC>
 int run_write(const KvMoveArgs<const T, C> &a, hipStream_t stream) {
-  // One token to a workgroup fills the chip soonest; from 4096 tokens on it is full anyway and the
-  // comparison with the following slots is what grows.
-  if (a.tokens < 4096)
-    return launch(kv_cache_write_kernel<T, C, D, VEC, 1>, dim3(a.tokens), dim3(256), 0, stream, a);
-  return launch(kv_cache_write_kernel<T, C, D, VEC, 16>, dim3((a.tokens + 15) / 16), dim3(256), 0, stream, a);
+  // Launches of 8192 tokens at most: the comparison grows with their square (131072 tokens, 8 heads of 128:
+  // 617 us in one launch, 314 so; 16384: 38 either way), and a later launch writes after an earlier one, as
+  // its tokens have to.
+  KvMoveArgs<const T, C> part = a;
+  for (part.first = 0; part.first < a.tokens; part.first = part.end) {
+    part.end = a.tokens - part.first > 8192 ? part.first + 8192 : a.tokens;
+    const int n = part.end - part.first;
+    // One token to a workgroup where that fills the chip less than once (48 tokens: 3.4 us, with four 5.2);
+    // more where there are more workgroups than places (4096: 9.5 with two, 11.0 with one or four; 8191:
+    // 15.6 with four, 16.7 with two, 20.4 with one).
+    const int e = n < 2048 ? launch(kv_cache_write_kernel<T, C, D, VEC, 1>, dim3(n), dim3(256), 0, stream, part)
+                  : n < 6144 ? launch(kv_cache_write_kernel<T, C, D, VEC, 2>, dim3((n + 1) / 2), dim3(256), 0, stream, part)
+                             : launch(kv_cache_write_kernel<T, C, D, VEC, 4>, dim3((n + 3) / 4), dim3(256), 0, stream, part);
+    if (e) return e;
+  }
+  return KCG_OK;
 }
 
 template <typename T, typename C, int D, bool VEC>
 int run_read(const KvMoveArgs<T, C> &a, hipStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(a.tokens) * 2 * a.cache.shape.heads, per = 256 / (D / 8);
-  return launch(kv_cache_read_kernel<T, C, D, VEC>, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), 0,
-                stream, a);
+  const int per = 256 / (D / 8), rows = 2 * a.cache.shape.heads;
+  // two rows to a lane (32768 tokens, 8 heads of 128, e4m3 to bf16: 54 us with one, 47 with two or four)
+  int group = 2 * per / rows;
+  if (group < 1) group = 1;
+  return launch(kv_cache_read_kernel<T, C, D, VEC, 2>, dim3((a.tokens + group - 1) / group), dim3(256), 0, stream, a, group);
 }
 
 template <bool WRITE, typename T, typename C>
@@ -137,7 +207,7 @@ int move(const kcg_kv_cache &cache, const kcg_rows &k, const kcg_rows &v, int dt
          hipStream_t stream) {
   const bool vec = rows_aligned16(k, dtype, B, S, cache.heads) && rows_aligned16(v, dtype, B, S, cache.heads);
   using U = std::conditional_t<WRITE, const T, T>;
-  const KvMoveArgs<U, C> a = {make_rows<U>(k), make_rows<U>(v), make_cache<C>(cache), slots, S, B * S};
+  const KvMoveArgs<U, C> a = {make_rows<U>(k), make_rows<U>(v), make_cache<C>(cache), slots, S, B * S, 0, 0};
 #define KCG_PICK(DD, V)                                         \
   if constexpr (WRITE) return run_write<T, C, DD, V>(a, stream); \
   else return run_read<T, C, DD, V>(a, stream)

@@ -81,7 +81,7 @@ __device__ __forceinline__ void rotate(float (&y)[8], const float (&cs)[8], cons
   }
 }
 
-template <typename T, int D, bool VEC, bool INTERLEAVED>
+template <typename T, int D, bool VEC, bool INTERLEAVED, bool STREAM>
 __global__ __launch_bounds__(64 * kNrWaves) void qk_norm_rope_kernel(const NormRopeArgs<T> a) {
   constexpr int LANES = D / 8, PER = 64 / LANES;  // rows that a wave holds at a time
   __shared__ float turns[kNrWaves][128];
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(64 * kNrWaves) void qk_norm_rope_kernel(const NormR
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = x[j] * r * (is_q ? wq[j] : wk[j]);
     rotate<D, INTERLEAVED>(x, cs, sn, a.rot, lane);
-    if (live) store8<VEC>(is_q ? a.q_out.at(b, s, row) + e0 : a.k_out.at(b, s, row - a.Hq) + e0, x);
+    if (live) store8<VEC, STREAM>(is_q ? a.q_out.at(b, s, row) + e0 : a.k_out.at(b, s, row - a.Hq) + e0, x);
   }
 }
 
@@ -184,19 +184,31 @@ __global__ __launch_bounds__(64 * kNrWaves) void qk_norm_rope_backward_kernel(co
   }
 }
 
-// Adds the workgroups' shares: 16 columns to a workgroup, 16 threads to a column.
+// Adds the workgroups' shares: 16 columns to a workgroup, 64 threads to a column, so that the up to 16
+// loads of a thread are under way together (1024 shares of 256 columns: 20 us with 16 threads to a
+// column, 4 with 64).
 template <typename T, int D>
-__global__ __launch_bounds__(256) void qk_norm_rope_weight_sum_kernel(const float *__restrict__ partial, int groups,
-                                                                      T *__restrict__ gq, T *__restrict__ gk) {
-  __shared__ float sums[16][17];
+__global__ __launch_bounds__(1024) void qk_norm_rope_weight_sum_kernel(const float *__restrict__ partial, int groups,
+                                                                       T *__restrict__ gq, T *__restrict__ gk) {
+  __shared__ float sums[64][17];
   const int c = threadIdx.x % 16, r = threadIdx.x / 16;
   const int column = blockIdx.x * 16 + c;
   float t = 0.0f;
-  for (int i = r; i < groups; i += 16) t += partial[static_cast<int64_t>(i) * 2 * D + column];
+#pragma unroll 8
+  for (int i = r; i < groups; i += 64) t += partial[static_cast<int64_t>(i) * 2 * D + column];
   sums[r][c] = t;
   __syncthreads();
+  if (r < 8) {
+    t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += sums[8 * i + r][c];
+  }
+  __syncthreads();
+  if (r < 8) sums[r][c] = t;
+  __syncthreads();
   if (r == 0) {
-    for (int i = 1; i < 16; ++i) t += sums[i][c];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) t += sums[i][c];
     T *to = column < D ? gq + column : gk + column - D;
     if constexpr (sizeof(T) == 4) *to = t;
     else *to = float_to_bf16(t);
@@ -261,13 +273,17 @@ int run_norm_rope(const NormRopeArgs<T> &a, T *gq, T *gk, hipStream_t stream) {
   const int64_t items = static_cast<int64_t>(a.tokens) * a.units;
   if (!a.partial) {
     const unsigned grid = static_cast<unsigned>((items + kNrWaves - 1) / kNrWaves);
-    return launch(qk_norm_rope_kernel<T, D, VEC, INTERLEAVED>, dim3(grid), dim3(64 * kNrWaves), 0, stream, a);
+    // Outputs of the last-level cache's size (256 MiB) and more go past it: 16384 tokens of 64 heads of 128 in
+    // bf16 take 100 us so, 106 otherwise; half as many 55 and 48.
+    if (VEC && static_cast<int64_t>(a.tokens) * a.rows * D * static_cast<int64_t>(sizeof(T)) >= int64_t{256} << 20)
+      return launch(qk_norm_rope_kernel<T, D, VEC, INTERLEAVED, VEC>, dim3(grid), dim3(64 * kNrWaves), 0, stream, a);
+    return launch(qk_norm_rope_kernel<T, D, VEC, INTERLEAVED, false>, dim3(grid), dim3(64 * kNrWaves), 0, stream, a);
   }
   const int groups = backward_groups(items);
   if (const int e = launch(qk_norm_rope_backward_kernel<T, D, VEC, INTERLEAVED>, dim3(groups), dim3(64 * kNrWaves), 0,
                            stream, a))
     return e;
-  return launch(qk_norm_rope_weight_sum_kernel<T, D>, dim3(2 * D / 16), dim3(256), 0, stream, a.partial, groups, gq, gk);
+  return launch(qk_norm_rope_weight_sum_kernel<T, D>, dim3(2 * D / 16), dim3(1024), 0, stream, a.partial, groups, gq, gk);
 }
 
 template <typename T>

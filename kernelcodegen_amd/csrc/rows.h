@@ -66,40 +66,59 @@ __device__ __forceinline__ void load8(const uint16_t *p, float (&x)[8]) {
     for (int j = 0; j < 8; ++j) x[j] = bf16_to_float(p[j]);
   }
 }
-template <bool VEC>
+// STREAM: past the caches, for outputs larger than them that nothing reads at once
+template <bool STREAM, typename V>
+__device__ __forceinline__ void store_vector(V x, void *p) {
+  if (STREAM) __builtin_nontemporal_store(x, static_cast<V *>(p));
+  else *static_cast<V *>(p) = x;
+}
+template <bool VEC, bool STREAM = false>
 __device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
   if (VEC) {
-    *reinterpret_cast<float4_t *>(p) = float4_t{x[0], x[1], x[2], x[3]};
-    *reinterpret_cast<float4_t *>(p + 4) = float4_t{x[4], x[5], x[6], x[7]};
+    store_vector<STREAM>(float4_t{x[0], x[1], x[2], x[3]}, p);
+    store_vector<STREAM>(float4_t{x[4], x[5], x[6], x[7]}, p + 4);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) p[j] = x[j];
   }
 }
-template <bool VEC>
+template <bool VEC, bool STREAM = false>
 __device__ __forceinline__ void store8(uint16_t *p, const float (&x)[8]) {
   if (VEC) {
     uint4_t a;
 #pragma unroll
     for (int j = 0; j < 4; ++j) a[j] = float_to_bf16_pair(x[2 * j], x[2 * j + 1]);
-    *reinterpret_cast<uint4_t *>(p) = a;
+    store_vector<STREAM>(a, p);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) p[j] = float_to_bf16(x[j]);
   }
 }
 
-// Sum (maximum) over the LANES lanes that hold a row.
+// x of another lane, in registers: lane ^ 1, lane ^ 2, 7 - lane of eight, 15 - lane of sixteen.
+template <int CTRL, typename T>
+__device__ __forceinline__ T from_lane(T x) {
+  return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kMirror8 = 0x141, kMirror16 = 0x140;
+
+// Sum (maximum) over the 8 or 16 lanes that hold a row; every lane gets it, in one order.
 template <int LANES>
 __device__ __forceinline__ float row_sum(float x) {
-#pragma unroll
-  for (int m = 1; m < LANES; m *= 2) x += __shfl_xor(x, m);
+  static_assert(LANES == 8 || LANES == 16, "lanes of a row");
+  x += from_lane<kXor1>(x);
+  x += from_lane<kXor2>(x);
+  x += from_lane<kMirror8>(x);
+  if (LANES == 16) x += from_lane<kMirror16>(x);
   return x;
 }
 template <int LANES>
-__device__ __forceinline__ float row_max(float x) {
-#pragma unroll
-  for (int m = 1; m < LANES; m *= 2) x = fmaxf(x, __shfl_xor(x, m));
+__device__ __forceinline__ unsigned row_max(unsigned x) {
+  static_assert(LANES == 8 || LANES == 16, "lanes of a row");
+  x = max(x, from_lane<kXor1>(x));
+  x = max(x, from_lane<kXor2>(x));
+  x = max(x, from_lane<kMirror8>(x));
+  if (LANES == 16) x = max(x, from_lane<kMirror16>(x));
   return x;
 }
 

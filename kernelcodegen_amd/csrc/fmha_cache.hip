@@ -122,8 +122,8 @@ __device__ __forceinline__ bool find_unit(const FmhaCacheArgs<C> &a, int unit, F
   return false;
 }
 
-// What a chunk looks like in LDS.  C: element of the cache.
-template <typename C, int D>
+// What a chunk looks like in LDS.  C: element of the cache; QT: 32-row tiles of queries to a wave.
+template <typename C, int D, int QT>
 struct FcTile {
   static constexpr int kRow = D * static_cast<int>(sizeof(C));  // bytes
   static constexpr int kPieces = kRow / 16;
@@ -131,12 +131,19 @@ struct FcTile {
   static constexpr int kRowsPerLoad = 64 / kPieces;             // one wave-wide direct load: 1024 bytes
   static constexpr int kLoads = kFcChunk / kRowsPerLoad;
   static constexpr int kBytes = kFcChunk * kRow;                // K, or V
-  static constexpr int kBuffer = 2 * kBytes + (sizeof(C) == 1 ? 256 : 0);  // K, V, exponents
-  static constexpr int kLoadsPerChunk = 2 * kLoads + (sizeof(C) == 1 ? 1 : 0);
-  static constexpr int kRing = 2 * kFcWaves * kBuffer;
-  static constexpr int kJoinRow = D + 4;                        // floats; padded
+  // LDS of a wave: a buffer of K, one of V, two of exponents (K's and V's)
+  static constexpr int kExps = sizeof(C) == 1 ? 256 : 0;
+  static constexpr int kWave = 2 * kBytes + 2 * kExps;
+  static constexpr int kLoadsK = kLoads + (kExps ? 1 : 0), kLoadsV = kLoads;
+  static constexpr int kJoinRow = 64 + 4;                       // floats; padded
   static constexpr int kJoin = kFcWaves * 32 * kJoinRow * 4;
-  static constexpr int kLds = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kStream = kFcWaves * kWave > kJoin ? kFcWaves * kWave : kJoin;
+  // The last kQLds steps of Q are kept in LDS where the accumulators of two tiles leave no registers for them:
+  // all of them, or as many as let two workgroups share a CU's 160 KiB.
+  static constexpr int kQLds = D * QT < 256 ? 0 : sizeof(C) == 1 ? 8 : 5;
+  static constexpr int kQ = QT * kQLds * 64 * 16;
+  static constexpr int kStats = 2 * kFcWaves * 32 * QT * 4;
+  static constexpr int kLds = kStream + kQ + kStats;
   static_assert(kRowsPerLoad <= 16, "a load stays inside a page");
 
   // K: 16 consecutive rows, one piece each
@@ -184,8 +191,8 @@ __device__ __forceinline__ bool not_finite(uint16_t x) { return (x & 0x7f80) == 
 // Q rows of the tile: 32 * QT columns of the products; TERMS: bf16 numbers that a weight is split over.
 // Two waves to a SIMD where the registers (or a bf16 chunk's LDS) allow it.
 template <typename C, int D, int QT, int TERMS>
-__global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || sizeof(C) == 2) ? 1 : 2)) void fmha_cache_kernel(const FmhaCacheArgs<C> a) {
-  using T = FcTile<C, D>;
+__global__ __launch_bounds__(64 * kFcWaves, 2) void fmha_cache_kernel(const FmhaCacheArgs<C> a) {
+  using T = FcTile<C, D, QT>;
   constexpr bool E8 = sizeof(C) == 1;
   constexpr int DT = D / 32, DS = D / 16;
   extern __shared__ __align__(16) uint8_t lds[];
@@ -234,50 +241,52 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
     return p >= 0 && p < a.cache.shape.pages ? p : -1;
   };
 
-  uint8_t *ring = lds + wave * 2 * T::kBuffer;
+  uint8_t *ring = lds + wave * T::kWave;
   const unsigned ring_at = __builtin_amdgcn_readfirstlane(lds_address(ring));
-  const int load_row = lane / T::kPieces;
-  int valid[2] = {0, 0};  // per buffer: bit g: the page of keys 16 g .. 16 g + 15 is the cache's
-  auto load_chunk = [&](int chunk, int buffer) {
+  constexpr int kV = T::kBytes, kX = 2 * kV;  // where V's buffer and the exponents' begin
+  const int load_row = lane / T::kPieces, load_pos = lane % T::kPieces;
+  // A chunk's rows: the cache rows of its first and its second 16 keys (of page 0 where the cache does not have
+  // their page), and bit g: it has the page of keys 16 g .. 16 g + 15.
+  int64_t base0 = 0, base1 = 0;
+  int ok = 0, next_ok = 0;
+  auto locate = [&](int chunk) {
     const int key0 = chunk * kFcChunk;
     const int p0 = page_of(key0), p1 = page_of(key0 + 16);
-    const int ok = (p0 >= 0 ? 1 : 0) | (p1 >= 0 ? 2 : 0);
-    if (buffer) valid[1] = ok;
-    else valid[0] = ok;
     const int in_page = (1 << log2_page) - 1;
-    const int64_t base[2] = {kv_row(a.cache.shape, max(p0, 0), head, key0 & in_page),
-                             kv_row(a.cache.shape, max(p1, 0), head, (key0 + 16) & in_page)};
-    const unsigned to = ring_at + buffer * T::kBuffer;
-    // the buffer's last reads are done (their results are used), as far as the hardware is told
+    next_ok = (p0 >= 0 ? 1 : 0) | (p1 >= 0 ? 2 : 0);
+    base0 = kv_row(a.cache.shape, max(p0, 0), head, key0 & in_page);
+    base1 = kv_row(a.cache.shape, max(p1, 0), head, (key0 + 16) & in_page);
+  };
+  // Requests the K (V) of the chunk located last, number n of this wave.  Whatever was read from the buffer has
+  // been used; the wait says so to the hardware as well.
+  auto load = [&](int n, bool is_v) {
+    const unsigned to = ring_at + (is_v ? kV : 0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    // byte offsets of this lane's pieces from the first row of a load; computed for each chunk, since
-    // registers are scarcer than these few instructions
-    int l_row = load_row, l_pos = lane % T::kPieces;
-    asm volatile("" : "+v"(l_row), "+v"(l_pos));
 #pragma unroll
     for (int j = 0; j < T::kLoads; ++j) {
       const int first = j * T::kRowsPerLoad;
-      const int64_t row = base[first / 16] + first % 16;
-      direct_load_16B(a.cache.k + row * D, l_row * T::kRow + (l_pos ^ T::swizzle_k(first + l_row)) * 16, to + j * 1024);
-      direct_load_16B(a.cache.v + row * D, l_row * T::kRow + (l_pos ^ T::swizzle_v(first + l_row)) * 16,
-                      to + T::kBytes + j * 1024);
+      const int swizzle = is_v ? T::swizzle_v(first + load_row) : T::swizzle_k(first + load_row);
+      direct_load_16B((is_v ? a.cache.v : a.cache.k) + ((first < 16 ? base0 : base1) + first % 16) * D,
+                      load_row * T::kRow + (load_pos ^ swizzle) * 16, to + j * 1024);
     }
-    if constexpr (E8) {
+    if (E8 && !is_v) {
       // dwords 0-7: K's exponents, 8-15: V's (the other lanes repeat them)
       const int i = lane & 7;
-      const uint8_t *from = (lane & 8 ? a.cache.v_exp : a.cache.k_exp) + (i < 4 ? base[0] : base[1]) + 4 * (i & 3);
-      direct_load_4B(from, to + 2 * T::kBytes);
+      direct_load_4B((lane & 8 ? a.cache.v_exp : a.cache.k_exp) + (i < 4 ? base0 : base1) + 4 * (i & 3),
+                     ring_at + kX + (n & 1) * T::kExps);
     }
   };
 
-  if (begin < end) load_chunk(begin, 0);
-  if (begin + 1 < end) load_chunk(begin + 1, 1);
+  if (begin < end) {
+    locate(begin);
+    load(0, false);
+    load(0, true);
+  }
 
   // ---- Q ----
-  // The last QL steps of Q are kept in LDS where the accumulators of two tiles leave no registers for them.
-  constexpr int QL = D * QT == 256 && E8 && TERMS == 1 ? 5 : 0;
-  __shared__ uint4_t q_lds[QL ? QT : 1][QL ? QL : 1][QL ? 64 : 1];
-  bf16x8_v q[QT][DS - QL];
+  constexpr int QL = T::kQLds;
+  uint4_t *q_lds = reinterpret_cast<uint4_t *>(lds + T::kStream);  // [QT][QL][64]
+  bf16x8_v q[QT][DS - QL ? DS - QL : 1];
   // Columns beyond the last row repeat it: what they compute is never stored.
   const int last_row = u.len.queries * a.group - 1;
 #pragma unroll
@@ -301,13 +310,12 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[s][j] ^= a.q_flip;
       if (s < DS - QL) q[t][s] = __builtin_bit_cast(bf16x8_v, x[s]);
-      else if (wave == (s - (DS - QL)) % kFcWaves) q_lds[QL ? t : 0][QL ? s - (DS - QL) : 0][QL ? lane : 0] = x[s];
+      else if (wave == (s - (DS - QL)) % kFcWaves) q_lds[(t * QL + s - (DS - QL)) * 64 + lane] = x[s];
     }
   }
   if (QL) __syncthreads();
   auto q_of = [&](int t, int s) {
-    return s < DS - QL ? q[t][s < DS - QL ? s : 0]
-                       : __builtin_bit_cast(bf16x8_v, q_lds[QL ? t : 0][QL ? s - (DS - QL) : 0][QL ? lane : 0]);
+    return s < DS - QL ? q[t][s < DS - QL ? s : 0] : __builtin_bit_cast(bf16x8_v, q_lds[(t * QL + s - (DS - QL)) * 64 + lane]);
   };
 
   float16_t acc[QT][DT];
@@ -322,23 +330,22 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
       for (int e = 0; e < 16; ++e) acc[t][i][e] = 0.0f;
   }
 
-  for (int chunk = begin; chunk < end; ++chunk) {
-    const int buffer = (chunk - begin) & 1;
-    if (chunk + 1 < end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::kLoadsPerChunk) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const uint8_t *ks = ring + buffer * T::kBuffer;
-    uint8_t *vs = ring + buffer * T::kBuffer + T::kBytes;
-    const uint8_t *xs = vs + T::kBytes;
-    // The lane's addresses; where registers are scarce they are computed for each chunk.
-    int at = lane;
-    if (QL) asm volatile("" : "+v"(at));
-    const int k_row = at & 31, k_half = at >> 5;
-    // V: row and byte column of this lane's transposing reads, within 16 keys and 32 columns
-    const int l16 = at & 15, side = (at >> 4) & 1;
-    const int v_row = E8 ? 4 * k_half + ((l16 >> 1) & 3) + 8 * (l16 >> 3) : 4 * k_half + (l16 >> 2);
-    const int v_piece = E8 ? side : 2 * side + ((l16 & 3) >> 1);
-    const int v_at = v_row * T::kRow + (l16 & 1) * 8;
+  // V: row and byte column of this lane's transposing reads, within 16 keys and 32 columns
+  const int l16 = lane & 15, side = (lane >> 4) & 1;
+  const int v_row = E8 ? 4 * half + ((l16 >> 1) & 3) + 8 * (l16 >> 3) : 4 * half + (l16 >> 2);
+  const int v_piece = E8 ? side : 2 * side + ((l16 & 3) >> 1);
+  const int v_at = v_row * T::kRow + (l16 & 1) * 8;
 
+  for (int chunk = begin; chunk < end; ++chunk) {
+    // Requests run K, V, K, V ...: while the scores of a chunk are computed its V is under way, while the weights
+    // and the output are, the next K.
+    const int n = chunk - begin;
+    const bool more = chunk + 1 < end;
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::kLoadsV) : "memory");
+    const uint8_t *ks = ring;
+    uint8_t *vs = ring + kV;
+    const uint8_t *xs = ring + kX + (n & 1) * T::kExps;
+    ok = next_ok;
     // ---- S^T = K . Q^T ----
     float16_t s[QT];
 #pragma unroll
@@ -346,10 +353,10 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
     if constexpr (E8) {
-      const float scale = exponent_to_scale(xs[k_row]);
+      const float scale = exponent_to_scale(xs[r32]);
 #pragma unroll
       for (int p = 0; p < D / 32; ++p) {
-        const uint4_t x = *reinterpret_cast<const uint4_t *>(ks + k_row * T::kRow + ((2 * p + k_half) ^ T::swizzle_k(k_row)) * 16);
+        const uint4_t x = *reinterpret_cast<const uint4_t *>(ks + r32 * T::kRow + ((2 * p + half) ^ T::swizzle_k(r32)) * 16);
         const bf16x8_v k0 = to_bf16(x[0], x[1], scale), k1 = to_bf16(x[2], x[3], scale);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
@@ -360,20 +367,25 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
     } else {
 #pragma unroll
       for (int p = 0; p < DS; ++p) {
-        const uint4_t x = *reinterpret_cast<const uint4_t *>(ks + k_row * T::kRow + ((2 * p + k_half) ^ T::swizzle_k(k_row)) * 16);
+        const uint4_t x = *reinterpret_cast<const uint4_t *>(ks + r32 * T::kRow + ((2 * p + half) ^ T::swizzle_k(r32)) * 16);
         const bf16x8_v k = __builtin_bit_cast(bf16x8_v, x);
 #pragma unroll
         for (int t = 0; t < QT; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q_of(t, p), s[t], 0, 0, 0);
       }
     }
 
+    if (more) {
+      locate(chunk + 1);
+      load(n + 1, false);
+    }
+
     // ---- masks ----
     const int key0 = chunk * kFcChunk;
-    const int ok = buffer ? valid[1] : valid[0];
-    if (key0 + kFcChunk > u.len.context || ok != 3) {
-      const unsigned there = (ok & 1 ? 0x0000ffffu : 0u) | (ok & 2 ? 0xffff0000u : 0u);
+    const bool masked = key0 + kFcChunk > u.len.context || ok != 3;
+    const unsigned there = (ok & 1 ? 0x0000ffffu : 0u) | (ok & 2 ? 0xffff0000u : 0u);
+    unsigned vis[QT];  // of a masked chunk: the keys that this lane's query sees
+    if (masked) {
       const int d0 = key0 - u.len.context;  // the first key's place among the drafts
-      unsigned vis[QT];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
         const int node = min(row0 + 32 * t + r32, last_row) / a.group;
@@ -388,6 +400,75 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
         for (int e = 0; e < 16; ++e)
           if (!((mine >> (8 * (e / 4) + e % 4)) & 1)) s[t][e] = -INFINITY;
       }
+    }
+
+    // ---- maxima ----
+    float neg[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      // The first maximum is the compiler's: it knows how long a product's result takes, the assembly
+      // of max3 does not, and each max3 needs the one before.
+      float top = fmaxf(s[t][0], s[t][1]);
+#pragma unroll
+      for (int e = 2; e < 16; e += 2) top = max3(top, s[t][e], s[t][e + 1]);
+      top *= a.c;
+      top = max_across_halves(top);
+      if (top > m[t] + kFcTau) {
+        const float keep = __builtin_amdgcn_exp2f(m[t] - top);  // 0 the first time
+        m[t] = top;
+        l[t] *= keep;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[t][i][e] *= keep;
+      }
+      neg[t] = m[t] == -INFINITY ? 0.0f : -m[t];
+    }
+
+    // ---- weights of 16 keys ----
+    unsigned p[QT][2][TERMS][4];  // bf16 pairs
+    auto weigh = [&](int kb) {
+      unsigned x[2] = {};
+      if constexpr (E8) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)  // V's exponents of the keys 16 kb + 8 g + 4 half .. + 3, less 128
+          x[g] = *reinterpret_cast<const unsigned *>(xs + 32 + 16 * kb + 8 * g + 4 * half) ^ 0x80808080u;
+      }
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int w2 = 0; w2 < 4; ++w2) {
+          float y[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) y[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * kb + 2 * w2 + k], a.c, neg[t]));
+          if (TERMS == 1) {
+            // the sum of the weights as they are rounded: what rounding does to one key alone cancels
+            const bf16_pair_t ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+            l[t] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16_pair_t, float_to_bf16_pair(y[0], y[1])), ones,
+                                                   l[t], false);
+          } else {
+            l[t] += y[0] + y[1];
+          }
+          if constexpr (E8) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              y[k] = __builtin_ldexpf(y[k], static_cast<int>(x[w2 / 2] << (24 - 8 * (2 * (w2 % 2) + k))) >> 24);
+          }
+#pragma unroll
+          for (int z = 0; z < TERMS; ++z) {
+            const unsigned pair = float_to_bf16_pair(y[0], y[1]);
+            p[t][kb][z][w2] = pair;
+            y[0] -= __builtin_bit_cast(float, pair << 16);
+            y[1] -= __builtin_bit_cast(float, pair & 0xffff0000u);
+          }
+        }
+    };
+    weigh(0);
+
+    // ---- V ----
+    if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::kLoadsK) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (masked) {
       // keys that some query may see; the rows of the others are zeroed
       const int left = keys - key0;
       const unsigned some = (left >= 32 ? 0xffffffffu : (1u << left) - 1) & there;
@@ -439,8 +520,7 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
       }
     }
 
-    // ---- V^T of the first 16 keys, before the weights are computed: an LDS read takes longer than the
-    // products between two ----
+    // all its reads before the first product: one takes longer than the products between two
     constexpr int kWords = E8 ? 2 : 4;
     unsigned v_raw[2][DT][kWords];
     auto read_v = [&](int kb) {
@@ -464,71 +544,13 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
           v_raw[kb][i][3] = hi[1];
         }
       }
-      asm volatile("" ::: "memory");  // (or the compiler moves the reads down to their uses)
     };
     read_v(0);
-
-    // ---- weights ----
-    unsigned p[QT][TERMS][8];  // bf16 pairs: elements 2w, 2w + 1
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      // The first maximum is the compiler's: it knows how long a product's result takes, the assembly
-      // of max3 does not, and each max3 needs the one before.
-      float top = fmaxf(s[t][0], s[t][1]);
-#pragma unroll
-      for (int e = 2; e < 16; e += 2) top = max3(top, s[t][e], s[t][e + 1]);
-      top *= a.c;
-      top = max_across_halves(top);
-      if (top > m[t] + kFcTau) {
-        const float keep = __builtin_amdgcn_exp2f(m[t] - top);  // 0 the first time
-        m[t] = top;
-        l[t] *= keep;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[t][i][e] *= keep;
-      }
-      const float neg = m[t] == -INFINITY ? 0.0f : -m[t];
-      unsigned x[4] = {};
-      if constexpr (E8) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g)  // V's exponents of the keys 8 g + 4 half .. + 3, less 128
-          x[g] = *reinterpret_cast<const unsigned *>(xs + 32 + 8 * g + 4 * k_half) ^ 0x80808080u;
-      }
-#pragma unroll
-      for (int w2 = 0; w2 < 8; ++w2) {
-        float y[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) y[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][2 * w2 + k], a.c, neg));
-        if (TERMS == 1) {
-          // the sum of the weights as they are rounded: what rounding does to one key alone cancels
-          const bf16_pair_t ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
-          l[t] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16_pair_t, float_to_bf16_pair(y[0], y[1])), ones,
-                                                 l[t], false);
-        } else {
-          l[t] += y[0] + y[1];
-        }
-        if constexpr (E8) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int e = 2 * w2 + k;
-            y[k] = __builtin_ldexpf(y[k], static_cast<int>(x[e / 4] << (24 - 8 * (e % 4))) >> 24);
-          }
-        }
-#pragma unroll
-        for (int z = 0; z < TERMS; ++z) {
-          const unsigned pair = float_to_bf16_pair(y[0], y[1]);
-          p[t][z][w2] = pair;
-          y[0] -= __builtin_bit_cast(float, pair << 16);
-          y[1] -= __builtin_bit_cast(float, pair & 0xffff0000u);
-        }
-      }
-    }
-
-    // ---- O^T += V^T . P^T ----
     read_v(1);
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    asm volatile("" ::: "memory");  // (or the compiler moves the reads down to their uses)
+
+    // ---- O^T += V^T . P^T; the other weights are computed between the products of the first 16 keys ----
+    auto multiply = [&](int kb) {
 #pragma unroll
       for (int i = 0; i < DT; ++i) {
         bf16x8_v v;
@@ -538,71 +560,83 @@ __global__ __launch_bounds__(64 * kFcWaves, (D * QT == 256 && (TERMS == 3 || siz
         for (int t = 0; t < QT; ++t)
 #pragma unroll
           for (int z = 0; z < TERMS; ++z) {
-            const uint4_t y = {p[t][z][4 * kb], p[t][z][4 * kb + 1], p[t][z][4 * kb + 2], p[t][z][4 * kb + 3]};
+            const uint4_t y = {p[t][kb][z][0], p[t][kb][z][1], p[t][kb][z][2], p[t][kb][z][3]};
             acc[t][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8_v, y), acc[t][i], 0, 0, 0);
           }
       }
-    if (chunk + 2 < end) load_chunk(chunk + 2, buffer);
+    };
+    multiply(0);
+    weigh(1);
+    multiply(1);
+    if (more) load(n + 1, true);
   }
 
-  // ---- join the waves ----
+  // ---- join the waves: 64 columns of 32 rows at a time ----
   float *join = reinterpret_cast<float *>(lds);
-  __shared__ float stats[2][kFcWaves][32 * QT];
+  float *stats_m = reinterpret_cast<float *>(lds + T::kStream + T::kQ);  // [waves][32 * QT]
+  float *stats_l = stats_m + kFcWaves * 32 * QT;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     l[t] += __shfl_xor(l[t], 32);
     if (half == 0) {
-      stats[0][wave][32 * t + r32] = m[t];
-      stats[1][wave][32 * t + r32] = l[t];
+      stats_m[wave * 32 * QT + 32 * t + r32] = m[t];
+      stats_l[wave * 32 * QT + 32 * t + r32] = l[t];
     }
   }
   const bool whole = u.count == 1;
   const int64_t slot = (static_cast<int64_t>(unit) * heads + head) * a.tiles + tile;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    __syncthreads();  // statistics are there; ring buffers and the last round's outputs are done with
-    float top = -INFINITY, sum = 0.0f;
+    float norm = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kFcWaves; ++k) top = fmaxf(top, stats[0][k][32 * t + r32]);
-    const float ref = top == -INFINITY ? 0.0f : top;
+    for (int part = 0; part < D / 64; ++part) {
+      __syncthreads();  // statistics are there; ring buffers and the last round's outputs are done with
+      if (part == 0) {
+        const int row = 32 * t + r32;
+        float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kFcWaves; ++k)
-      sum += stats[1][k][32 * t + r32] * __builtin_amdgcn_exp2f(stats[0][k][32 * t + r32] - ref);
-    // (e4m3: the weights were 2^-1 of what they stand for)
-    const float norm = (sum == 0.0f ? 0.0f : (E8 ? 2.0f : 1.0f) / sum) * __builtin_amdgcn_exp2f(m[t] - ref);
-    float *mine = join + (wave * 32 + r32) * T::kJoinRow + 4 * half;
+        for (int k = 0; k < kFcWaves; ++k) top = fmaxf(top, stats_m[k * 32 * QT + row]);
+        const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float16_t &x = acc[t][i];
-        *reinterpret_cast<float4_t *>(mine + 32 * i + 8 * g) =
-            float4_t{x[4 * g] * norm, x[4 * g + 1] * norm, x[4 * g + 2] * norm, x[4 * g + 3] * norm};
+        for (int k = 0; k < kFcWaves; ++k)
+          sum += stats_l[k * 32 * QT + row] * __builtin_amdgcn_exp2f(stats_m[k * 32 * QT + row] - ref);
+        // (e4m3: the weights were 2^-1 of what they stand for)
+        norm = (sum == 0.0f ? 0.0f : (E8 ? 2.0f : 1.0f) / sum) * __builtin_amdgcn_exp2f(m[t] - ref);
+        if (!whole && wave == 0 && half == 0 && row < a.rows)
+          a.partial[a.logs + slot * a.rows + row] = sum == 0.0f ? -INFINITY : ref + __builtin_amdgcn_logf(sum);
       }
-    const int row = 32 * t + r32;
-    if (!whole && wave == 0 && half == 0 && row < a.rows)
-      a.partial[a.logs + slot * a.rows + row] = sum == 0.0f ? -INFINITY : ref + __builtin_amdgcn_logf(sum);
-    __syncthreads();
-    for (int i = threadIdx.x; i < 32 * (D / 4); i += 64 * kFcWaves) {
-      const int r = i / (D / 4), d = 4 * (i % (D / 4));
-      const int at = row0 + 32 * t + r, node = at / a.group, h = head * a.group + at - node * a.group;
-      if (node >= u.len.queries) break;
-      float4_t y = {};
+      float *mine = join + (wave * 32 + r32) * T::kJoinRow + 4 * half;
 #pragma unroll
-      for (int k = 0; k < kFcWaves; ++k) y += *reinterpret_cast<const float4_t *>(join + (k * 32 + r) * T::kJoinRow + d);
-      if (!whole) {
-        *reinterpret_cast<float4_t *>(a.partial + (slot * a.rows + 32 * t + r) * D + d) = y;
-      } else if constexpr (TERMS == 1) {
-        uint16_t *to = static_cast<uint16_t *>(a.out.data) + b * a.out.stride_b + node * a.out.stride_s + h * a.out.stride_h + d;
-        const uint2_t z = {float_to_bf16_pair(y[0], y[1]), float_to_bf16_pair(y[2], y[3])};
-        if (a.vec) *reinterpret_cast<uint2_t *>(to) = z;
-        else
-          for (int j = 0; j < 4; ++j) to[j] = float_to_bf16(y[j]);
-      } else {
-        float *to = static_cast<float *>(a.out.data) + b * a.out.stride_b + node * a.out.stride_s + h * a.out.stride_h + d;
-        if (a.vec) *reinterpret_cast<float4_t *>(to) = y;
-        else
-          for (int j = 0; j < 4; ++j) to[j] = y[j];
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float16_t &x = acc[t][2 * part + i];
+          *reinterpret_cast<float4_t *>(mine + 32 * i + 8 * g) =
+              float4_t{x[4 * g] * norm, x[4 * g + 1] * norm, x[4 * g + 2] * norm, x[4 * g + 3] * norm};
+        }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = 16 * i + threadIdx.x / 16, column = 4 * (threadIdx.x % 16), d = 64 * part + column;
+        const int row = row0 + 32 * t + r, node = row / a.group, h = head * a.group + row - node * a.group;
+        if (node >= u.len.queries) break;
+        float4_t y = {};
+#pragma unroll
+        for (int k = 0; k < kFcWaves; ++k) y += *reinterpret_cast<const float4_t *>(join + (k * 32 + r) * T::kJoinRow + column);
+        if (!whole) {
+          *reinterpret_cast<float4_t *>(a.partial + (slot * a.rows + 32 * t + r) * D + d) = y;
+        } else if constexpr (TERMS == 1) {
+          uint16_t *to = static_cast<uint16_t *>(a.out.data) + b * a.out.stride_b + node * a.out.stride_s + h * a.out.stride_h + d;
+          const uint2_t z = {float_to_bf16_pair(y[0], y[1]), float_to_bf16_pair(y[2], y[3])};
+          if (a.vec) *reinterpret_cast<uint2_t *>(to) = z;
+          else
+            for (int j = 0; j < 4; ++j) to[j] = float_to_bf16(y[j]);
+        } else {
+          float *to = static_cast<float *>(a.out.data) + b * a.out.stride_b + node * a.out.stride_s + h * a.out.stride_h + d;
+          if (a.vec) *reinterpret_cast<float4_t *>(to) = y;
+          else
+            for (int j = 0; j < 4; ++j) to[j] = y[j];
+        }
       }
     }
   }
@@ -677,7 +711,7 @@ inline FcPlan plan_fmha_cache(const kcg_kv_cache &c, int width, int B, int N, in
   p.qt = p.rows_all <= 32 ? 1 : 2;
   p.tiles = (p.rows_all + 32 * p.qt - 1) / (32 * p.qt);
   p.rows = p.tiles > 1 ? 64 : p.rows_all;
-  p.places = c.dtype == KCG_E4M3 || c.dim == 64 ? 2 : 1;  // (a bf16 ring of 128 elements is 128 KiB)
+  p.places = 2;
   const int64_t per_unit = static_cast<int64_t>(c.heads) * p.tiles;
   const int64_t round = 256 * p.places / per_unit;  // units that run at once
   // A few sequences: one round, less the unit that each sequence's remainder may add (a tree of 32 over 131072
@@ -708,7 +742,7 @@ inline FcPlan plan_fmha_cache(const kcg_kv_cache &c, int width, int B, int N, in
 template <typename C, int D, int QT, int TERMS>
 int run_fmha_cache(FmhaCacheArgs<C> &a, bool split, hipStream_t stream) {
   const auto kernel = fmha_cache_kernel<C, D, QT, TERMS>;
-  const int lds = FcTile<C, D>::kLds;
+  const int lds = FcTile<C, D, QT>::kLds;
   if (!allow_lds(kernel, lds)) return KCG_ERR_LAUNCH;
   const int64_t items = static_cast<int64_t>(a.max_units) * a.cache.shape.heads;
   const int64_t grid = (items + kNumXcd - 1) / kNumXcd * kNumXcd * a.tiles;

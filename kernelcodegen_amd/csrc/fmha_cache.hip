@@ -94,7 +94,6 @@ __device__ __forceinline__ bool find_unit(const FmhaCacheArgs<C> &a, int unit, F
   }
   int64_t per = (total + a.want_units - 1) / a.want_units;
   per = per < kFcMinChunks ? kFcMinChunks : per > (1 << 30) ? 1 << 30 : per;  // (no sequence has as many)
-  u.chunks_per_unit = static_cast<int>(per);
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     if (a.B > 64) {  // (else they are still there)
@@ -112,6 +111,9 @@ __device__ __forceinline__ bool find_unit(const FmhaCacheArgs<C> &a, int unit, F
       u.count = __builtin_amdgcn_readlane(units, at);
       u.first = before + __builtin_amdgcn_readlane(upto, at) - u.count;
       u.index = unit - u.first;
+      // the sequence's units are of one size
+      const int all = __builtin_amdgcn_readlane(chunks, at);
+      u.chunks_per_unit = u.count ? (all + u.count - 1) / u.count : 0;
       u.len.context = __builtin_amdgcn_readlane(l.context, at);
       u.len.drafts = __builtin_amdgcn_readlane(l.drafts, at);
       u.len.queries = __builtin_amdgcn_readlane(l.queries, at);
@@ -715,10 +717,9 @@ inline FcPlan plan_fmha_cache(const kcg_kv_cache &c, int width, int B, int N, in
   const int64_t per_unit = static_cast<int64_t>(c.heads) * p.tiles;
   const int64_t round = 256 * p.places / per_unit;  // units that run at once
   // A few sequences: one round, less the unit that each sequence's remainder may add (a tree of 32 over 131072
-  // keys: 119 us, 130 with two rounds, 168 with four).  Many: rounds enough that the last one, which
-  // is not full, does not count for much (64 single tokens over contexts to 8192: 131 us with one, 120
-  // with 1.25 to 2.75, 124 with four).
-  int64_t want = 8 * B <= round ? round - B : 5 * round / 2;
+  // keys: 119 us, 130 with two rounds, 168 with four).  Many: one and a half (64 single tokens over contexts to
+  // 8192: 125 us with one, 120 with 1.5 to 2.5, 122 with 3.5; all over 4096: 110, 115, 116 and 121).
+  int64_t want = 8 * B <= round ? round - B : 3 * round / 2;
   if (want < 1) want = 1;
   const int64_t chunks = (static_cast<int64_t>(width) * c.page_size + kFcChunk - 1) / kFcChunk;
   const int64_t most = B * ((chunks + kFcMinChunks - 1) / kFcMinChunks);

@@ -134,9 +134,11 @@ def check(status):
 def raw_stream(index):
     """The current stream of device `index` as a number.  (torch.cuda.current_stream builds a
     Stream object for it, which takes as long as a small kernel.)"""
+    global raw_stream
     import torch
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return get(index) if get is not None else torch.cuda.current_stream(index).cuda_stream
+    raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda index: torch.cuda.current_stream(index).cuda_stream)
+    return raw_stream(index)
 
 
 def current_stream():

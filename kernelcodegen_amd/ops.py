@@ -187,19 +187,20 @@ def fmha(Q, K, V, scale=1.0, causal=False, out=None, out_dtype=None, sched=None)
 
 # A small call takes as long as its checks: each helper below first asks everything in one
 # expression and looks for what is wrong only where that fails.
+_Tensor, _contiguous, _pack_rows = torch.Tensor, torch.contiguous_format, lib.pack_rows
 
 
 def _rows(t, name, dtype, index, shape=None):
     """kcg_rows of a [B,S,H,D] (or [tokens,H,D]) tensor on device `index`: any strides but a
     contiguous last axis."""
-    if isinstance(t, torch.Tensor) and t.dtype == dtype and t.get_device() == index and (
+    if isinstance(t, _Tensor) and t.dtype == dtype and t.get_device() == index and (
             shape is None or t.shape == shape):
         stride = t.stride()
         if len(stride) == 4 and stride[3] == 1:
-            return lib.pack_rows(t.data_ptr(), stride[0], stride[1], stride[2])
+            return _pack_rows(t.data_ptr(), stride[0], stride[1], stride[2])
         if len(stride) == 3 and stride[2] == 1:
-            return lib.pack_rows(t.data_ptr(), 0, stride[0], stride[1])
-    if not isinstance(t, torch.Tensor) or t.dim() not in (3, 4):
+            return _pack_rows(t.data_ptr(), 0, stride[0], stride[1])
+    if not isinstance(t, _Tensor) or t.dim() not in (3, 4):
         raise ValueError("%s must be a [B,S,H,D] or [tokens,H,D] tensor" % name)
     if t.get_device() != index:
         raise ValueError("%s must be on device cuda:%d" % (name, index))
@@ -212,7 +213,7 @@ def _rows(t, name, dtype, index, shape=None):
 
 def _plain(t, name, dtype, shape, index):
     """Address of a contiguous tensor of this type and shape on device `index`."""
-    if not (isinstance(t, torch.Tensor) and t.dtype == dtype and t.get_device() == index and t.shape == shape
+    if not (isinstance(t, _Tensor) and t.dtype == dtype and t.get_device() == index and t.shape == shape
             and t.is_contiguous()):
         _check(t, name, dtype, shape, torch.device("cuda", index))
     return t.data_ptr()
@@ -241,11 +242,8 @@ def _workspace(workspace, need, index):
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
-_contiguous = torch.contiguous_format
-
-
 def _norm_rope_args(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved):
-    if not isinstance(q, torch.Tensor) or q.dtype not in _DTYPES or not q.is_cuda or q.dim() not in (3, 4):
+    if not isinstance(q, _Tensor) or q.dtype not in _DTYPES or not q.is_cuda or q.dim() not in (3, 4):
         raise ValueError("q must be a float32 or bfloat16 device tensor [B,S,H,D] or [tokens,H,D]")
     index, dtype = q.get_device(), q.dtype
     rq, rk = _rows(q, "q", dtype, index), _rows(k, "k", dtype, index)
@@ -253,7 +251,7 @@ def _norm_rope_args(q, k, q_weight, k_weight, positions, inv_freq, eps, interlea
     Hq, D = shape[-2:]
     if k_shape[:-2] != shape[:-2] or k_shape[-1] != D:
         raise ValueError("k must have q's tokens and head dimension")
-    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1:
+    if not isinstance(inv_freq, _Tensor) or inv_freq.dim() != 1:
         raise ValueError("inv_freq must be a tensor of one frequency for each rotated pair")
     pairs = inv_freq.shape[0]
     args = (_plain(q_weight, "q_weight", dtype, (D,), index), _plain(k_weight, "k_weight", dtype, (D,), index),
@@ -313,7 +311,7 @@ class KvCache:
     """
 
     def __init__(self, k, v, k_exp=None, v_exp=None):
-        if not isinstance(k, torch.Tensor) or k.dim() != 4 or not k.is_cuda:
+        if not isinstance(k, _Tensor) or k.dim() != 4 or not k.is_cuda:
             raise ValueError("k must be a [pages, heads, page_size, dim] device tensor")
         if k.dtype not in (torch.bfloat16, torch.float8_e4m3fn):
             raise ValueError("a cache holds bfloat16 or float8_e4m3fn, not %s" % k.dtype)
@@ -357,7 +355,7 @@ def kv_cache_write(cache, k, v, slots):
     rounded to the cache's type; kcg_kv_cache_write says how.
     """
     index = _cache_device(cache)
-    if not isinstance(k, torch.Tensor) or k.dtype not in _DTYPES:
+    if not isinstance(k, _Tensor) or k.dtype not in _DTYPES:
         raise ValueError("k must be a float32 or bfloat16 tensor")
     dtype, shape = k.dtype, k.shape
     rk, rv = _rows(k, "k", dtype, index), _rows(v, "v", dtype, index, shape)
@@ -374,7 +372,7 @@ def kv_cache_read(cache, slots, out_dtype=torch.bfloat16, out=None):
     strides but a contiguous last axis.
     """
     index = _cache_device(cache)
-    if not isinstance(slots, torch.Tensor) or slots.dim() not in (1, 2):
+    if not isinstance(slots, _Tensor) or slots.dim() not in (1, 2):
         raise ValueError("slots must be an int32 tensor [B,S] or [tokens]")
     shape = tuple(slots.shape)
     at = _plain(slots, "slots", torch.int32, shape, index)
@@ -387,7 +385,7 @@ def kv_cache_read(cache, slots, out_dtype=torch.bfloat16, out=None):
         v = torch.empty_like(k)
     else:
         k, v = out
-        out_dtype = k.dtype if isinstance(k, torch.Tensor) else None
+        out_dtype = k.dtype if isinstance(k, _Tensor) else None
         if out_dtype not in _DTYPES:
             raise ValueError("a cache is read as float32 or bfloat16")
     _call(lib.load().kcg_kv_cache_read, index, cache._c, at, _rows(k, "out[0]", out_dtype, index, shape),
@@ -412,14 +410,14 @@ def fmha_cache(q, cache, block_table, context_lens, draft_lens=None, tree_mask=N
     int32.  Rows of `out` from draft_lens[b] on stay as they were.  kcg_fmha_cache says the rest.
     """
     index = _cache_device(cache)
-    if not isinstance(q, torch.Tensor) or q.dim() != 4:
+    if not isinstance(q, _Tensor) or q.dim() != 4:
         raise ValueError("q must be a [B,N,H,dim] tensor")
     rq = _rows(q, "q", torch.bfloat16, index)
     shape = q.shape
     B, N, Hq, D = shape
     if D != cache.dim or Hq % cache.heads:
         raise ValueError("q must have the cache's dim and a multiple of its heads")
-    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
+    if not isinstance(block_table, _Tensor) or block_table.dim() != 2:
         raise ValueError("block_table must be an int32 tensor [B, pages]")
     width = block_table.shape[1]
     table = _plain(block_table, "block_table", torch.int32, (B, width), index)
@@ -429,7 +427,7 @@ def fmha_cache(q, cache, block_table, context_lens, draft_lens=None, tree_mask=N
     if out is None:
         out_dtype = out_dtype or torch.bfloat16
         out = (torch.empty if draft_lens is None else torch.zeros)(shape, dtype=out_dtype, device=q.device)
-    elif not isinstance(out, torch.Tensor) or out_dtype not in (None, out.dtype):
+    elif not isinstance(out, _Tensor) or out_dtype not in (None, out.dtype):
         raise ValueError("out must be a tensor of dtype out_dtype")
     out_dtype = out.dtype
     if out_dtype not in _DTYPES:

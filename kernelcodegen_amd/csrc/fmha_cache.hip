@@ -24,9 +24,10 @@
 //    masks.  There, V rows that nobody sees are zeroed in LDS (their weight is 0, and 0 * NaN is not),
 //    and values that are not finite are taken out of the product and added to the rows that see them.
 //  * How many chunks make a unit follows from the lengths, which are on the device: every wave sums
-//    them up and finds its unit (no host synchronisation, equal work for ragged batches).  A sequence
-//    that fits one unit is written at once; the others leave normalised partial outputs and the
-//    logarithms of their sums in the workspace, joined by a second launch.
+//    them up and finds its unit (no host synchronisation, equal work for ragged batches); for more than 64
+//    sequences a launch of one workgroup does that first.  A sequence that fits one unit is written at
+//    once; the others leave normalised partial outputs and the logarithms of their sums in the
+//    workspace, joined by a last launch.
 #include "kv_cache.h"
 
 namespace kcg {
@@ -34,6 +35,7 @@ namespace kcg {
 typedef __bf16 bf16x8_v __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4_v __attribute__((ext_vector_type(4)));
 typedef int int2_v __attribute__((ext_vector_type(2)));
+typedef int int4_v __attribute__((ext_vector_type(4)));
 
 constexpr int kFcWaves = 4;
 constexpr int kFcChunk = 32;      // keys to a chunk
@@ -47,18 +49,20 @@ struct FmhaCacheArgs {
   KvCache<C> cache;
   const int32_t *table, *context, *drafts;
   const uint64_t *tree;
-  float *partial;  // [unit][head][tile][rows][D], then the logarithms [unit][head][tile][rows]
+  float *partial;  // [slot][head][tile][rows][D], then the logarithms [slot][head][tile][rows]
   int64_t logs;    // where those begin, in floats
+  int4_v *sequences;  // for more than 64 sequences: first unit, units and first slot of each,
+  int32_t *unit_of;   // and the sequence of each unit, -1 behind the last one
   int B, N, Hq, width, group, tiles, rows, want_units, max_units;
   float c;
   unsigned q_flip;  // sign bits of two bf16 numbers, or 0
   bool vec;
 };
 
-// Chunks to a unit, and which unit of which sequence number `unit` is.
+// Unit `index` of the `count` of sequence b.  A sequence of several units has slots of the workspace from
+// `slot` on, one to a unit: units of sequences that are cut are at most twice the units wanted.
 struct FcUnit {
-  int b, index, count, first;  // unit `index` of the `count` of sequence b; `first`: the number of its unit 0
-  int chunks_per_unit;
+  int b, index, count, slot;
   KvLens len;
 };
 
@@ -79,49 +83,100 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-// Every wave does this for itself: the lengths of all sequences, 64 at a time.  Sequences without
-// queries have no unit, the others at least one.  With `unit` < 0 looks for sequence -1 - unit.
+__device__ __forceinline__ int fc_chunks(const KvLens &l) { return (l.context + l.drafts + kFcChunk - 1) / kFcChunk; }
+
+// Chunks to a unit at most, for `total` chunks of all sequences.
+__device__ __forceinline__ int fc_chunks_per_unit(int64_t total, int want_units) {
+  const int64_t per = (total + want_units - 1) / want_units;
+  return static_cast<int>(per < kFcMinChunks ? kFcMinChunks : per > (1 << 30) ? 1 << 30 : per);  // (none has as many)
+}
+
+// Sequences without queries have no unit, the others at least one.
+__device__ __forceinline__ int fc_units(const KvLens &l, int per) {
+  const int chunks = fc_chunks(l);
+  return !l.queries ? 0 : chunks <= per ? 1 : (chunks + per - 1) / per;
+}
+
+// Finds unit `unit`, or with `unit` < 0 the units of sequence -1 - unit; false: there is no such unit.  Up
+// to 64 sequences: every wave does it for itself, a sequence to a lane.
 template <typename C>
 __device__ __forceinline__ bool find_unit(const FmhaCacheArgs<C> &a, int unit, FcUnit &u) {
   const int lane = threadIdx.x & 63;
-  int64_t total = 0;
+  if (!a.want_units) {  // every sequence is one unit
+    u = {unit, 0, 1, 0, fc_lens(a, unit)};
+    return u.len.queries > 0;
+  }
+  if (a.B > 64) {
+    u.b = unit < 0 ? -1 - unit : a.unit_of[unit];
+    if (u.b < 0) return false;
+    const int4_v s = a.sequences[u.b];
+    u.index = unit - s[0];
+    u.count = s[1];
+    u.slot = s[2];
+    u.len = fc_lens(a, u.b);
+    return true;
+  }
   KvLens l = {0, 0, 0};
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    l = {0, 0, 0};
-    if (b0 + lane < a.B) l = fc_lens(a, b0 + lane);
-    const int chunks = l.queries ? (l.context + l.drafts + kFcChunk - 1) / kFcChunk : 0;
-    total += __builtin_amdgcn_readlane(wave_scan(chunks), 63);
+  if (lane < a.B) l = fc_lens(a, lane);
+  const int per = fc_chunks_per_unit(__builtin_amdgcn_readlane(wave_scan(l.queries ? fc_chunks(l) : 0), 63), a.want_units);
+  const int units = fc_units(l, per), upto = wave_scan(units), slots = wave_scan(units > 1 ? units : 0);
+  const uint64_t found = __ballot(unit >= 0 ? unit >= upto - units && unit < upto : lane == -1 - unit);
+  if (!found) return false;
+  u.b = __builtin_ctzll(found);
+  u.count = __builtin_amdgcn_readlane(units, u.b);
+  u.index = unit - __builtin_amdgcn_readlane(upto, u.b) + u.count;
+  u.slot = __builtin_amdgcn_readlane(slots, u.b) - u.count;
+  u.len.context = __builtin_amdgcn_readlane(l.context, u.b);
+  u.len.drafts = __builtin_amdgcn_readlane(l.drafts, u.b);
+  u.len.queries = __builtin_amdgcn_readlane(l.queries, u.b);
+  return true;
+}
+
+// One workgroup for more than 64 sequences, 1024 at a time.
+template <typename C>
+__global__ __launch_bounds__(1024) void fmha_cache_units_kernel(const FmhaCacheArgs<C> a) {
+  __shared__ int sums[2][16];
+  __shared__ unsigned long long total;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x == 0) total = 0;
+  __syncthreads();
+  int64_t mine = 0;
+  for (int b = threadIdx.x; b < a.B; b += 1024) {
+    const KvLens l = fc_lens(a, b);
+    if (l.queries) mine += fc_chunks(l);
   }
-  int64_t per = (total + a.want_units - 1) / a.want_units;
-  per = per < kFcMinChunks ? kFcMinChunks : per > (1 << 30) ? 1 << 30 : per;  // (no sequence has as many)
-  int before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    if (a.B > 64) {  // (else they are still there)
-      l = {0, 0, 0};
-      if (b0 + lane < a.B) l = fc_lens(a, b0 + lane);
+  if (mine) atomicAdd(&total, static_cast<unsigned long long>(mine));  // (whole numbers: any order)
+  __syncthreads();
+  const int per = fc_chunks_per_unit(static_cast<int64_t>(total), a.want_units);
+  int units_before = 0, slots_before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 1024) {
+    const int b = b0 + threadIdx.x;
+    int units = 0;
+    if (b < a.B) units = fc_units(fc_lens(a, b), per);
+    const int cut = units > 1 ? units : 0;
+    int first = wave_scan(units), slot = wave_scan(cut);
+    if (lane == 63) {
+      sums[0][wave] = first;
+      sums[1][wave] = slot;
     }
-    const int chunks = (l.context + l.drafts + kFcChunk - 1) / kFcChunk;
-    const int units = !l.queries ? 0 : chunks <= per ? 1 : (chunks + static_cast<int>(per) - 1) / static_cast<int>(per);
-    const int upto = wave_scan(units);
-    const bool mine = unit >= 0 ? units && unit >= before + upto - units && unit < before + upto : b0 + lane == -1 - unit;
-    const uint64_t found = __ballot(mine);
-    if (found) {
-      const int at = __builtin_ctzll(found);
-      u.b = b0 + at;
-      u.count = __builtin_amdgcn_readlane(units, at);
-      u.first = before + __builtin_amdgcn_readlane(upto, at) - u.count;
-      u.index = unit - u.first;
-      // the sequence's units are of one size
-      const int all = __builtin_amdgcn_readlane(chunks, at);
-      u.chunks_per_unit = u.count ? (all + u.count - 1) / u.count : 0;
-      u.len.context = __builtin_amdgcn_readlane(l.context, at);
-      u.len.drafts = __builtin_amdgcn_readlane(l.drafts, at);
-      u.len.queries = __builtin_amdgcn_readlane(l.queries, at);
-      return true;
+    __syncthreads();
+    first += units_before - units;
+    slot += slots_before - cut;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) {
+        first += sums[0][w];
+        slot += sums[1][w];
+      }
+      units_before += sums[0][w];
+      slots_before += sums[1][w];
     }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    if (b < a.B) {
+      a.sequences[b] = int4_v{first, units, slot, 0};
+      for (int i = 0; i < units; ++i) a.unit_of[first + i] = b;
+    }
+    __syncthreads();  // (sums are written again)
   }
-  return false;
+  for (int i = units_before + threadIdx.x; i < a.max_units; i += 1024) a.unit_of[i] = -1;
 }
 
 // What a chunk looks like in LDS.  C: element of the cache; QT: 32-row tiles of queries to a wave.
@@ -217,8 +272,8 @@ __global__ __launch_bounds__(64 * kFcWaves, 2) void fmha_cache_kernel(const Fmha
   // ---- this wave's chunks ----
   const int keys = u.len.context + u.len.drafts;
   const int chunks = (keys + kFcChunk - 1) / kFcChunk;
-  const int unit_begin = u.index * u.chunks_per_unit;
-  const int unit_end = min(chunks, unit_begin + u.chunks_per_unit);
+  const int per_unit = (chunks + u.count - 1) / u.count;  // a sequence's units are of one size
+  const int unit_begin = min(chunks, u.index * per_unit), unit_end = min(chunks, unit_begin + per_unit);
   const int per_wave = (unit_end - unit_begin + kFcWaves - 1) / kFcWaves;
   const int begin = min(unit_end, unit_begin + wave * per_wave), end = min(unit_end, begin + per_wave);
 
@@ -586,7 +641,7 @@ __global__ __launch_bounds__(64 * kFcWaves, 2) void fmha_cache_kernel(const Fmha
     }
   }
   const bool whole = u.count == 1;
-  const int64_t slot = (static_cast<int64_t>(unit) * heads + head) * a.tiles + tile;
+  const int64_t slot = (static_cast<int64_t>(u.slot + u.index) * heads + head) * a.tiles + tile;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     float norm = 0.0f;
@@ -658,9 +713,9 @@ __global__ __launch_bounds__(256) void fmha_cache_join_kernel(const FmhaCacheArg
   FcUnit u;
   if (!find_unit(a, -1 - b, u) || u.count < 2 || node >= u.len.queries) return;
   const int head = h / a.group, row = node * a.group + h - head * a.group;
-  const int tile = a.tiles == 1 ? 0 : row / 64, r = row - tile * 64;
+  const int tile = row / 64, r = row - tile * 64;  // (one tile holds at most 64 rows)
   const int64_t step = static_cast<int64_t>(a.cache.shape.heads) * a.tiles * a.rows;
-  const int64_t first = (static_cast<int64_t>(u.first) * a.cache.shape.heads + head) * a.tiles * a.rows +
+  const int64_t first = (static_cast<int64_t>(u.slot) * a.cache.shape.heads + head) * a.tiles * a.rows +
                         static_cast<int64_t>(tile) * a.rows + r;
   const float *logs = a.partial + a.logs + first;
   const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
@@ -700,56 +755,56 @@ __global__ __launch_bounds__(256) void fmha_cache_join_kernel(const FmhaCacheArg
 
 // How a call is split; the query and the call agree on it.
 struct FcPlan {
-  int group, rows_all, qt, tiles, rows;  // rows: of a tile that are stored
-  int places;                            // workgroups that a CU holds
-  int want_units, max_units;
-  int64_t floats;  // workspace
+  int group, qt, tiles, rows;  // rows: of a tile that are stored
+  int want_units, max_units;   // want_units 0: one unit to a sequence, nothing is stored between
+  int64_t logs, sequences, unit_of, bytes;  // where the parts of the workspace begin, and its size
 };
 
 inline FcPlan plan_fmha_cache(const kcg_kv_cache &c, int width, int B, int N, int Hq, int64_t workspace_bytes) {
-  FcPlan p;
+  FcPlan p = {};
   p.group = Hq / c.heads;
-  p.rows_all = N * p.group;
-  p.qt = p.rows_all <= 32 ? 1 : 2;
-  p.tiles = (p.rows_all + 32 * p.qt - 1) / (32 * p.qt);
-  p.rows = p.tiles > 1 ? 64 : p.rows_all;
-  p.places = 2;
+  const int rows = N * p.group;
+  p.qt = rows <= 32 ? 1 : 2;
+  p.tiles = (rows + 32 * p.qt - 1) / (32 * p.qt);
+  p.rows = p.tiles > 1 ? 64 : rows;
+  p.max_units = B;
   const int64_t per_unit = static_cast<int64_t>(c.heads) * p.tiles;
-  const int64_t round = 256 * p.places / per_unit;  // units that run at once
+  const int64_t round = 2 * kNumCu / per_unit;  // units that run at once, two workgroups to a CU
   // A few sequences: one round, less the unit that each sequence's remainder may add (a tree of 32 over 131072
   // keys: 119 us, 130 with two rounds, 168 with four).  Many: one and a half (64 single tokens over contexts to
   // 8192: 125 us with one, 120 with 1.5 to 2.5, 122 with 3.5; all over 4096: 110, 115, 116 and 121).
-  int64_t want = 8 * B <= round ? round - B : 3 * round / 2;
-  if (want < 1) want = 1;
+  int64_t want = 8 * static_cast<int64_t>(B) <= round ? round - B : 3 * round / 2;
   const int64_t chunks = (static_cast<int64_t>(width) * c.page_size + kFcChunk - 1) / kFcChunk;
   const int64_t most = B * ((chunks + kFcMinChunks - 1) / kFcMinChunks);
   if (want > most) want = most;
-  const int64_t floats_per_unit = per_unit * p.rows * (c.dim + 1);
-  int64_t units = want + B;
-  if (workspace_bytes >= 0 && units > workspace_bytes / 4 / floats_per_unit) units = workspace_bytes / 4 / floats_per_unit;
-  if (chunks <= kFcMinChunks || units <= B) {
-    // one unit to a sequence: nothing is stored between
-    p.want_units = 0;
-    p.max_units = B;
-    p.floats = 0;
+  if (chunks <= kFcMinChunks) return p;
+  for (; want > 0; want /= 2) {  // (less, where the workspace does not hold what is preferred)
+    const int64_t slots = B < want ? want + B : 2 * want;  // see FcUnit
+    p.logs = slots * per_unit * p.rows * c.dim;
+    p.sequences = ((p.logs + slots * per_unit * p.rows) * 4 + 15) / 16 * 16;
+    p.unit_of = p.sequences + (B > 64 ? static_cast<int64_t>(B) * 16 : 0);
+    p.bytes = p.unit_of + (B > 64 ? (want + B) * 4 : 0);
+    if (workspace_bytes >= 0 && p.bytes > workspace_bytes) continue;
+    p.want_units = static_cast<int>(want);
+    p.max_units = static_cast<int>(want + B);
     return p;
   }
-  p.want_units = static_cast<int>(units - B);
-  p.max_units = static_cast<int>(units);
-  p.floats = units * floats_per_unit;
+  p.bytes = 0;
   return p;
 }
 
 template <typename C, int D, int QT, int TERMS>
-int run_fmha_cache(FmhaCacheArgs<C> &a, bool split, hipStream_t stream) {
+int run_fmha_cache(const FmhaCacheArgs<C> &a, hipStream_t stream) {
   const auto kernel = fmha_cache_kernel<C, D, QT, TERMS>;
   const int lds = FcTile<C, D, QT>::kLds;
   if (!allow_lds(kernel, lds)) return KCG_ERR_LAUNCH;
   const int64_t items = static_cast<int64_t>(a.max_units) * a.cache.shape.heads;
   const int64_t grid = (items + kNumXcd - 1) / kNumXcd * kNumXcd * a.tiles;
   if (grid > 0x7fffffffLL) return KCG_ERR_UNSUPPORTED_SHAPE;
+  if (a.want_units && a.B > 64)
+    if (const int e = launch(fmha_cache_units_kernel<C>, dim3(1), dim3(1024), 0, stream, a)) return e;
   if (const int e = launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * kFcWaves), lds, stream, a)) return e;
-  if (!split) return KCG_OK;
+  if (!a.want_units) return KCG_OK;
   const int64_t rows = static_cast<int64_t>(a.B) * a.N * a.Hq;
   using O = std::conditional_t<TERMS == 1, uint16_t, float>;
   return launch(fmha_cache_join_kernel<C, D, O>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, a);
@@ -760,7 +815,6 @@ int fmha_cache(const kcg_rows &q, const kcg_kv_cache &cache, const int32_t *tabl
                const int32_t *drafts, const uint64_t *tree, const kcg_rows &out, int o_dtype, int B, int N, int Hq,
                float scale, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
   const FcPlan p = plan_fmha_cache(cache, width, B, N, Hq, workspace ? workspace_bytes : 0);
-  const bool split = p.want_units > 0;
   FmhaCacheArgs<C> a = {};
   a.q = make_rows<const uint16_t>(q);
   a.out = make_rows<void>(out);
@@ -770,7 +824,11 @@ int fmha_cache(const kcg_rows &q, const kcg_kv_cache &cache, const int32_t *tabl
   a.drafts = drafts;
   a.tree = tree;
   a.partial = static_cast<float *>(workspace);
-  a.logs = static_cast<int64_t>(p.max_units) * cache.heads * p.tiles * p.rows * cache.dim;
+  a.logs = p.logs;
+  if (p.want_units && B > 64) {
+    a.sequences = reinterpret_cast<int4_v *>(static_cast<char *>(workspace) + p.sequences);
+    a.unit_of = reinterpret_cast<int32_t *>(static_cast<char *>(workspace) + p.unit_of);
+  }
   a.B = B;
   a.N = N;
   a.Hq = Hq;
@@ -778,7 +836,7 @@ int fmha_cache(const kcg_rows &q, const kcg_kv_cache &cache, const int32_t *tabl
   a.group = p.group;
   a.tiles = p.tiles;
   a.rows = p.rows;
-  a.want_units = split ? p.want_units : 1;
+  a.want_units = p.want_units;
   a.max_units = p.max_units;
   // The scale's sign goes into Q, so that the maximum of the scores is that of the products.  For a scale
   // of 0 the smallest normal number stands: its products vanish beside 1, and -inf stays -inf under it.
@@ -786,7 +844,7 @@ int fmha_cache(const kcg_rows &q, const kcg_kv_cache &cache, const int32_t *tabl
   a.c = scale == 0.0f ? 1.17549435e-38f : fabsf(scale) * 1.44269504088896340736f;
   a.vec = rows_aligned16(q, KCG_BF16, B, N, Hq) && rows_aligned16(out, o_dtype, B, N, Hq);
 #define KCG_PICK(DD, QQ) \
-  return o_dtype == KCG_F32 ? run_fmha_cache<C, DD, QQ, 3>(a, split, stream) : run_fmha_cache<C, DD, QQ, 1>(a, split, stream)
+  return o_dtype == KCG_F32 ? run_fmha_cache<C, DD, QQ, 3>(a, stream) : run_fmha_cache<C, DD, QQ, 1>(a, stream)
   if (cache.dim == 64) {
     if (p.qt == 1) { KCG_PICK(64, 1); }
     KCG_PICK(64, 2);
@@ -811,7 +869,7 @@ extern "C" {
 
 int64_t kcg_fmha_cache_ws_bytes(const kcg_kv_cache *cache, int32_t table_width, int32_t B, int32_t N, int32_t Hq) {
   if (kcg::check_fmha_cache(cache, table_width, B, N, Hq)) return 0;
-  return kcg::plan_fmha_cache(*cache, table_width, B, N, Hq, -1).floats * 4;
+  return kcg::plan_fmha_cache(*cache, table_width, B, N, Hq, -1).bytes;
 }
 
 int kcg_fmha_cache(const kcg_rows *q, const kcg_kv_cache *cache, const int32_t *block_table, int32_t table_width,

@@ -477,6 +477,47 @@ def test_fmha_cache_large_scores(dev):
         check_fmha(dev, cache, q, table, [638], None, None, 30.0, F32)
 
 
+@pytest.mark.parametrize("B, longest", [(65, 3000), (130, 700), (1100, 300)])
+def test_fmha_cache_many_sequences(dev, B, longest):
+    """More sequences than lanes: empty ones, ones without drafts, a few long ones among short ones."""
+    N, Hq, Hk, D, page = 2, 2, 1, 64, 16
+    g = gen(B)
+    context = torch.randint(0, 40, (B,), generator=g)
+    context[::9] = 0
+    context[3], context[B // 2], context[B - 1] = longest, longest // 2, longest - 17
+    drafts = torch.randint(0, N + 1, (B,), generator=g)
+    drafts[3] = drafts[B - 1] = N
+    per = -(-(longest + N) // page)
+    cache = filled_cache(dev, per + 50, Hk, page, D, BF16)
+    table = torch.randint(0, per + 50, (B, per), generator=g).to(torch.int32)
+    q = normal(1, B, N, Hq, D, dtype=BF16)
+    for workspace in (None, torch.empty(200000, dtype=torch.uint8, device=dev)):
+        check_fmha(dev, cache, q, table, context.tolist(), drafts.tolist(), None, 0.125, F32, workspace=workspace)
+
+
+def test_fmha_cache_no_queries_at_all(dev):
+    for B in (3, 100):
+        cache = filled_cache(dev, 64, 2, 16, 128, E4M3)
+        q = normal(1, B, 2, 4, 128, dtype=BF16)
+        table = torch.zeros(B, 64, dtype=torch.int32)
+        check_fmha(dev, cache, q, table, [900] * B, [0] * B, None, 1.0, BF16)
+
+
+@pytest.mark.parametrize("power", [-90, 60])
+def test_fmha_cache_exponents_far_from_one(dev, power):
+    """V's powers of two go through the weights: rows of very small and very large values, and both together."""
+    cache = filled_cache(dev, 8, 1, 16, 64, E4M3)
+    cache.v_exp.add_(power)
+    cache.v_exp[::2] -= 7
+    q = normal(1, 1, 3, 2, 64, dtype=BF16)
+    for out_dtype in (BF16, F32):
+        check_fmha(dev, cache, q, make_table(1, 8, 8, 2), [120], None, None, 0.1, out_dtype)
+    # K's: scores of 2^power times the queries' 2^-power
+    cache = filled_cache(dev, 8, 1, 16, 64, E4M3)
+    cache.k_exp.add_(power)
+    check_fmha(dev, cache, (q.float() * 2.0 ** -power).to(BF16), make_table(1, 8, 8, 2), [120], None, None, 0.1, F32)
+
+
 def test_fmha_cache_query_layouts(dev):
     """Queries inside a fused projection, in [B,H,N,D] memory and of no alignment; outputs likewise; no workspace."""
     B, N, Hq, Hk, D = 2, 3, 6, 2, 128

@@ -281,8 +281,9 @@ typedef struct kcg_rows {
  * rot_dim on are not rotated.  q is [B][S][Hq][D], k [B][S][Hk][D], positions [B][S] and
  * inv_freq [rot_dim / 2] contiguous; everything but inv_freq (fp32) and positions (int32) is of
  * `dtype` (KCG_F32 or KCG_BF16).  Arithmetic is fp32 (angles: 64 bits), one rounding at the end.
- * D is 64 or 128; rot_dim a multiple of 16 from 16 to D.  An output may be its own input (same
- * data and strides); otherwise outputs overlap no input. */
+ * D is 64 or 128; rot_dim a multiple of 16 from 16 to D; eps 0 or more (below the smallest normal number it
+ * counts as that).  An output may be its own input (same data and strides); otherwise outputs
+ * overlap no input and not each other. */
 KCG_API int kcg_qk_norm_rope(const kcg_rows *q, const kcg_rows *k, const kcg_rows *q_out,
                              const kcg_rows *k_out, const void *q_weight, const void *k_weight,
                              const int32_t *positions, const float *inv_freq, int dtype, int32_t B,
@@ -308,7 +309,7 @@ KCG_API int kcg_qk_norm_rope_backward(const kcg_rows *dq, const kcg_rows *dk, co
                                       int64_t workspace_bytes, void *stream);
 
 /* A paged key/value cache: k and v are [pages][heads][page_size][dim] of KCG_BF16 or KCG_E4M3.
- * An e4m3 row stands for its values times 2^(x - 127), x its byte in k_exp / v_exp
+ * An e4m3 row stands for its values times 2^(x - 127), x its byte (1 to 254) in k_exp / v_exp
  * [pages][heads][page_size] (NULL for bf16).  A power of two keeps every dequantised value a
  * bf16 number.  page_size is 16, 32, 64, 128 or 256, dim 64 or 128; all pointers 16-byte
  * aligned.  A token's slot is page * page_size + its place in the page. */

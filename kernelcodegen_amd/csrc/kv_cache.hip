@@ -68,7 +68,8 @@ __device__ __forceinline__ void cache_store8(uint8_t *to, uint8_t *exponent, flo
 // GROUP tokens to a workgroup, all their heads.  A token that names the same slot as a later one is
 // left out, so that the last one is what the slot holds, whichever workgroup runs first: the
 // workgroup compares its GROUP slots with all that follow.  That is 4 bytes read per following
-// token and workgroup (2 tokens^2 / GROUP bytes, from L2); the first rows are on their way meanwhile.
+// token and workgroup (2 tokens^2 / GROUP bytes, from L2); the first rows are on their way meanwhile
+// (later ones ahead of their turn gained nothing: the chip is full of waves).
 template <typename T, typename C, int D, bool VEC, int GROUP>
 __global__ __launch_bounds__(256) void kv_cache_write_kernel(const KvMoveArgs<const T, C> a) {
   constexpr int LANES = D / 8, PER = 256 / LANES;
@@ -112,22 +113,18 @@ __global__ __launch_bounds__(256) void kv_cache_write_kernel(const KvMoveArgs<co
   for (; t < end; t += 256) compare(t, a.slots[t]);
   __syncthreads();
   while (g < count) {
-    int next_g = g + step_g, next_r = r + step_r;
-    if (next_r >= rows) {
-      next_r -= rows;
-      ++next_g;
-    }
-    float next[8];
-    if (next_g < count) load(next_g, next_r, next);
     const bool is_v = r >= heads;
     const int64_t row = later[g] ? -1 : kv_slot_row(a.cache.shape, a.slots[t0 + g], is_v ? r - heads : r);
     if (row >= 0)
       cache_store8<LANES>((is_v ? a.cache.v : a.cache.k) + row * D + 8 * lane,
                           (is_v ? a.cache.v_exp : a.cache.k_exp) + row, x, lane);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = next[j];
-    g = next_g;
-    r = next_r;
+    g += step_g;
+    r += step_r;
+    if (r >= rows) {
+      r -= rows;
+      ++g;
+    }
+    if (g < count) load(g, r, x);
   }
 }
 
@@ -176,15 +173,15 @@ __global__ __launch_bounds__(256) void kv_cache_read_kernel(const KvMoveArgs<T, 
 template <typename T, typename C, int D, bool VEC>
 int run_write(const KvMoveArgs<const T, C> &a, hipStream_t stream) {
   // Launches of 8192 tokens at most: the comparison grows with their square (131072 tokens, 8 heads of 128:
-  // 617 us in one launch, 314 so; 16384: 38 either way), and a later launch writes after an earlier one, as
+  // 617 us in one launch, 300 so; 16384: 35 to 38), and a later launch writes after an earlier one, as
   // its tokens have to.
   KvMoveArgs<const T, C> part = a;
   for (part.first = 0; part.first < a.tokens; part.first = part.end) {
     part.end = a.tokens - part.first > 8192 ? part.first + 8192 : a.tokens;
     const int n = part.end - part.first;
-    // One token to a workgroup where that fills the chip less than once (48 tokens: 3.4 us, with four 5.2);
-    // more where there are more workgroups than places (4096: 9.5 with two, 11.0 with one or four; 8191:
-    // 15.6 with four, 16.7 with two, 20.4 with one).
+    // One token to a workgroup where that fills the chip less than once (64 tokens: 3.5 us, with four 4.9);
+    // more where there are more workgroups than places (4096: 9.0 with two, 9.8 with four, 11.6 with one;
+    // 8191: 14.7 with four, 16.1 with two, 20.8 with one).
     const int e = n < 2048 ? launch(kv_cache_write_kernel<T, C, D, VEC, 1>, dim3(n), dim3(256), 0, stream, part)
                   : n < 6144 ? launch(kv_cache_write_kernel<T, C, D, VEC, 2>, dim3((n + 1) / 2), dim3(256), 0, stream, part)
                              : launch(kv_cache_write_kernel<T, C, D, VEC, 4>, dim3((n + 3) / 4), dim3(256), 0, stream, part);

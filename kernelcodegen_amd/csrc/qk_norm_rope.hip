@@ -104,7 +104,7 @@ __global__ __launch_bounds__(64 * kNrWaves) void qk_norm_rope_kernel(const NormR
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(x[j], x[j], sum);
-    const float r = 1.0f / sqrtf(row_sum<LANES>(sum) * (1.0f / D) + a.eps);
+    const float r = __builtin_amdgcn_rsqf(row_sum<LANES>(sum) * (1.0f / D) + a.eps);
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = x[j] * r * (is_q ? wq[j] : wk[j]);
     rotate<D, INTERLEAVED>(x, cs, sn, a.rot, lane);
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(64 * kNrWaves) void qk_norm_rope_backward_kernel(co
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(x[j], x[j], sum);
-      const float r = 1.0f / sqrtf(row_sum<LANES>(sum) * (1.0f / D) + a.eps);
+      const float r = __builtin_amdgcn_rsqf(row_sum<LANES>(sum) * (1.0f / D) + a.eps);
       float dot = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -244,7 +244,7 @@ NormRopeArgs<T> norm_rope_args(int B, int S, int Hq, int Hk, int D, int rot, flo
   a.rows = Hq + Hk;
   a.rot = rot;
   a.tokens = B * S;
-  a.eps = eps;
+  a.eps = eps < 1.17549435e-38f ? 1.17549435e-38f : eps;  // (v_rsq_f32 takes no subnormal numbers)
   const int u = norm_rope_units(a.tokens, a.rows, D);
   a.unit_rows = unit_rows(a.rows, u, D);
   a.units = (a.rows + a.unit_rows - 1) / a.unit_rows;

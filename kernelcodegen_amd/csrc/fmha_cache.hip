@@ -40,6 +40,7 @@ typedef int int4_v __attribute__((ext_vector_type(4)));
 constexpr int kFcWaves = 4;
 constexpr int kFcChunk = 32;      // keys to a chunk
 constexpr int kFcMinChunks = 4;   // of a unit: one to a wave
+constexpr int kFcWhole = 24;      // where no sequence can have more, none is cut
 constexpr float kFcTau = 8.0f;    // log2 by which a maximum may lag behind before the sums are rescaled
 
 template <typename C>
@@ -54,6 +55,7 @@ struct FmhaCacheArgs {
   int4_v *sequences;  // for more than 64 sequences: first unit, units and first slot of each,
   int32_t *unit_of;   // and the sequence of each unit, -1 behind the last one
   int B, N, Hq, width, group, tiles, rows, want_units, max_units;
+  bool few;        // sequences, so that each may have many units
   float c;
   unsigned q_flip;  // sign bits of two bf16 numbers, or 0
   bool vec;
@@ -85,16 +87,17 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 __device__ __forceinline__ int fc_chunks(const KvLens &l) { return (l.context + l.drafts + kFcChunk - 1) / kFcChunk; }
 
-// Chunks to a unit at most, for `total` chunks of all sequences.
+// Chunks to a unit, for `total` chunks of all sequences.
 __device__ __forceinline__ int fc_chunks_per_unit(int64_t total, int want_units) {
   const int64_t per = (total + want_units - 1) / want_units;
-  return static_cast<int>(per < kFcMinChunks ? kFcMinChunks : per > (1 << 30) ? 1 << 30 : per);  // (none has as many)
+  return static_cast<int>(per < kFcMinChunks ? kFcMinChunks : per > (1 << 28) ? 1 << 28 : per);  // (none has as many)
 }
 
-// Sequences without queries have no unit, the others at least one.
+// Sequences without queries have no unit, the others at least one.  A sequence a little longer than a unit is
+// left whole.
 __device__ __forceinline__ int fc_units(const KvLens &l, int per) {
   const int chunks = fc_chunks(l);
-  return !l.queries ? 0 : chunks <= per ? 1 : (chunks + per - 1) / per;
+  return !l.queries ? 0 : 4 * chunks < 5 * per ? 1 : (chunks + per - 1) / per;
 }
 
 // Finds unit `unit`, or with `unit` < 0 the units of sequence -1 - unit; false: there is no such unit.  Up
@@ -246,9 +249,9 @@ __device__ __forceinline__ bool not_finite(uint8_t x) { return (x & 0x7f) == 0x7
 __device__ __forceinline__ bool not_finite(uint16_t x) { return (x & 0x7f80) == 0x7f80; }
 
 // Q rows of the tile: 32 * QT columns of the products; TERMS: bf16 numbers that a weight is split over.
-// Two waves to a SIMD where the registers (or a bf16 chunk's LDS) allow it.
+// Two waves to a SIMD; three (168 registers) with one tile, where that spills nothing.
 template <typename C, int D, int QT, int TERMS>
-__global__ __launch_bounds__(64 * kFcWaves, 2) void fmha_cache_kernel(const FmhaCacheArgs<C> a) {
+__global__ __launch_bounds__(64 * kFcWaves, QT == 1 && (D == 64 || TERMS == 1) ? 3 : 2) void fmha_cache_kernel(const FmhaCacheArgs<C> a) {
   using T = FcTile<C, D, QT>;
   constexpr bool E8 = sizeof(C) == 1;
   constexpr int DT = D / 32, DS = D / 16;
@@ -699,50 +702,57 @@ __global__ __launch_bounds__(64 * kFcWaves, 2) void fmha_cache_kernel(const Fmha
   }
 }
 
-// Joins the units of the sequences that have several: a workgroup to an output row, D / 4 lanes of
-// float4 to a unit's share of it, so that 1024 / D units are on their way at a time.
+// Joins the units of the sequences that have several, D / 4 lanes of float4 to a unit's share of a row.  Few
+// sequences: a workgroup to a row, 1024 / D units under way at a time.  Many: a workgroup to 1024 / D rows of
+// a sequence, since each has few units if any, and finding them takes longer than joining them.
 template <typename C, int D, typename O>
 __global__ __launch_bounds__(256) void fmha_cache_join_kernel(const FmhaCacheArgs<C> a) {
   constexpr int LANES = D / 4, GROUPS = 256 / LANES;
   __shared__ float4_t shares[GROUPS][LANES];
   __shared__ float sums[GROUPS];
-  const int lane = threadIdx.x & 63;
-  const int per_sequence = a.N * a.Hq;
-  const int b = blockIdx.x / per_sequence, at = blockIdx.x - b * per_sequence;
-  const int node = at / a.Hq, h = at - node * a.Hq;
+  const int per_sequence = a.N * a.Hq, parts = a.few ? per_sequence : (per_sequence + GROUPS - 1) / GROUPS;
+  const int b = blockIdx.x / parts, part = blockIdx.x - b * parts;
   FcUnit u;
-  if (!find_unit(a, -1 - b, u) || u.count < 2 || node >= u.len.queries) return;
+  if (!find_unit(a, -1 - b, u) || u.count < 2) return;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, d = 4 * lane;
+  const int at = a.few ? part : part * GROUPS + group;  // row of the sequence
+  const int node = at / a.Hq, h = at - node * a.Hq;
+  const bool live = node < u.len.queries && at < per_sequence;
+  if (a.few && !live) return;
   const int head = h / a.group, row = node * a.group + h - head * a.group;
   const int tile = row / 64, r = row - tile * 64;  // (one tile holds at most 64 rows)
   const int64_t step = static_cast<int64_t>(a.cache.shape.heads) * a.tiles * a.rows;
   const int64_t first = (static_cast<int64_t>(u.slot) * a.cache.shape.heads + head) * a.tiles * a.rows +
                         static_cast<int64_t>(tile) * a.rows + r;
-  const float *logs = a.partial + a.logs + first;
-  const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
-  // the first shares are on their way while the logarithms are looked through
-  float4_t y = {}, next = {};
-  if (group < u.count) next = *reinterpret_cast<const float4_t *>(a.partial + (first + group * step) * D + d);
-  float top = -INFINITY;
-  for (int i = lane; i < u.count; i += 64) top = fmaxf(top, logs[i * step]);
-#pragma unroll
-  for (int k = 1; k < 64; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
+  const float *logs = a.partial + a.logs + first, *share = a.partial + first * D + d;
+  float top = -INFINITY, sum = 0.0f;
+  float4_t y = {};
+  if (live)
+#pragma unroll 4
+    for (int i = 0; i < u.count; ++i) top = fmaxf(top, logs[i * step]);
   const float ref = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f;
-  for (int i = group; i < u.count; i += GROUPS) {
-    const float4_t x = next;
-    if (i + GROUPS < u.count) next = *reinterpret_cast<const float4_t *>(a.partial + (first + (i + GROUPS) * step) * D + d);
+  auto add = [&](int i) {
     const float weight = __builtin_amdgcn_exp2f(logs[i * step] - ref);
+    const float4_t x = *reinterpret_cast<const float4_t *>(share + i * step * D);
     sum += weight;
 #pragma unroll
     for (int j = 0; j < 4; ++j) y[j] = __builtin_fmaf(weight, x[j], y[j]);
-  }
-  shares[group][threadIdx.x % LANES] = y;
-  if (d == 0) sums[group] = sum;
-  __syncthreads();
-  if (group) return;
-  for (int k = 1; k < GROUPS; ++k) {  // (in a fixed order)
-    y += shares[k][threadIdx.x];
-    sum += sums[k];
+  };
+  if (!a.few) {
+    if (!live) return;
+#pragma unroll 4
+    for (int i = 0; i < u.count; ++i) add(i);
+  } else {
+#pragma unroll 4
+    for (int i = group; i < u.count; i += GROUPS) add(i);
+    shares[group][lane] = y;
+    if (lane == 0) sums[group] = sum;
+    __syncthreads();
+    if (group) return;
+    for (int k = 1; k < GROUPS; ++k) {  // (in a fixed order)
+      y += shares[k][lane];
+      sum += sums[k];
+    }
   }
   y *= sum == 0.0f ? 0.0f : 1.0f / sum;
   O *to = static_cast<O *>(a.out.data) + b * a.out.stride_b + node * a.out.stride_s + h * a.out.stride_h + d;
@@ -757,6 +767,7 @@ __global__ __launch_bounds__(256) void fmha_cache_join_kernel(const FmhaCacheArg
 struct FcPlan {
   int group, qt, tiles, rows;  // rows: of a tile that are stored
   int want_units, max_units;   // want_units 0: one unit to a sequence, nothing is stored between
+  bool few;
   int64_t logs, sequences, unit_of, bytes;  // where the parts of the workspace begin, and its size
 };
 
@@ -770,14 +781,15 @@ inline FcPlan plan_fmha_cache(const kcg_kv_cache &c, int width, int B, int N, in
   p.max_units = B;
   const int64_t per_unit = static_cast<int64_t>(c.heads) * p.tiles;
   const int64_t round = 2 * kNumCu / per_unit;  // units that run at once, two workgroups to a CU
-  // A few sequences: one round, less the unit that each sequence's remainder may add (a tree of 32 over 131072
-  // keys: 119 us, 130 with two rounds, 168 with four).  Many: one and a half (64 single tokens over contexts to
-  // 8192: 125 us with one, 120 with 1.5 to 2.5, 122 with 3.5; all over 4096: 110, 115, 116 and 121).
-  int64_t want = 8 * static_cast<int64_t>(B) <= round ? round - B : 3 * round / 2;
+  // A few sequences: one round, less the unit that each one's remainder may add (a tree of 32 over 131072
+  // keys: 119 us, with two rounds 130, with four 168).  Many: one and a half, since lengths differ (64
+  // single tokens over contexts to 8192: 121 us, with one round 126; where they do not, 24 over 4000: 45 us,
+  // whole 44; 16: 35 and 42).
+  p.few = 8 * static_cast<int64_t>(B) <= round;
+  int64_t want = p.few ? round - B : 3 * round / 2;
   const int64_t chunks = (static_cast<int64_t>(width) * c.page_size + kFcChunk - 1) / kFcChunk;
-  const int64_t most = B * ((chunks + kFcMinChunks - 1) / kFcMinChunks);
-  if (want > most) want = most;
-  if (chunks <= kFcMinChunks) return p;
+  // (1 x 4 heads over 500 keys: 9.5 us whole, 10.4 in four units, and two launches more to ask for; 750: 11.4, 10.1)
+  if (chunks <= kFcWhole) return p;
   for (; want > 0; want /= 2) {  // (less, where the workspace does not hold what is preferred)
     const int64_t slots = B < want ? want + B : 2 * want;  // see FcUnit
     p.logs = slots * per_unit * p.rows * c.dim;
@@ -805,9 +817,10 @@ int run_fmha_cache(const FmhaCacheArgs<C> &a, hipStream_t stream) {
     if (const int e = launch(fmha_cache_units_kernel<C>, dim3(1), dim3(1024), 0, stream, a)) return e;
   if (const int e = launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(64 * kFcWaves), lds, stream, a)) return e;
   if (!a.want_units) return KCG_OK;
-  const int64_t rows = static_cast<int64_t>(a.B) * a.N * a.Hq;
+  const int64_t rows = static_cast<int64_t>(a.N) * a.Hq, groups = a.few ? 1 : 1024 / D;
   using O = std::conditional_t<TERMS == 1, uint16_t, float>;
-  return launch(fmha_cache_join_kernel<C, D, O>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, a);
+  return launch(fmha_cache_join_kernel<C, D, O>, dim3(static_cast<unsigned>(a.B * ((rows + groups - 1) / groups))), dim3(256),
+                0, stream, a);
 }
 
 template <typename C>
@@ -838,6 +851,7 @@ int fmha_cache(const kcg_rows &q, const kcg_kv_cache &cache, const int32_t *tabl
   a.rows = p.rows;
   a.want_units = p.want_units;
   a.max_units = p.max_units;
+  a.few = p.few;
   // The scale's sign goes into Q, so that the maximum of the scores is that of the products.  For a scale
   // of 0 the smallest normal number stands: its products vanish beside 1, and -inf stays -inf under it.
   a.q_flip = scale < 0.0f ? 0x80008000u : 0u;

@@ -211,6 +211,13 @@ def _rows(t, name, dtype, index, shape=None):
     raise ValueError("the last axis of %s must be contiguous" % name)
 
 
+def _new_rows(t):
+    """kcg_rows of a contiguous tensor that was made here."""
+    shape = t.shape
+    H, D = shape[-2], shape[-1]
+    return _pack_rows(t.data_ptr(), shape[-3] * H * D, H * D, D)
+
+
 def _plain(t, name, dtype, shape, index):
     """Address of a contiguous tensor of this type and shape on device `index`."""
     if not (isinstance(t, _Tensor) and t.dtype == dtype and t.get_device() == index and t.shape == shape
@@ -230,12 +237,12 @@ def _call(fn, index, *args):
         lib.check(st)
 
 
-def _workspace(workspace, need, index):
+def _workspace(workspace, need, index, device):
     """(address, bytes) of a workspace, and the tensor that holds it."""
     if workspace is None:
         if not need:
             return None, 0, None
-        workspace = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", index))
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
         return workspace.data_ptr(), need, workspace
     if not (isinstance(workspace, torch.Tensor) and workspace.get_device() == index and workspace.is_contiguous()):
         raise ValueError("workspace must be a contiguous tensor on cuda:%d" % index)
@@ -243,21 +250,25 @@ def _workspace(workspace, need, index):
 
 
 def _norm_rope_args(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved):
-    if not isinstance(q, _Tensor) or q.dtype not in _DTYPES or not q.is_cuda or q.dim() not in (3, 4):
-        raise ValueError("q must be a float32 or bfloat16 device tensor [B,S,H,D] or [tokens,H,D]")
+    if not isinstance(q, _Tensor) or not q.is_cuda:
+        raise ValueError("q must be a device tensor")
     index, dtype = q.get_device(), q.dtype
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise ValueError("q must be float32 or bfloat16, not %s" % dtype)
     rq, rk = _rows(q, "q", dtype, index), _rows(k, "k", dtype, index)
-    shape, k_shape = q.shape, k.shape
-    Hq, D = shape[-2:]
-    if k_shape[:-2] != shape[:-2] or k_shape[-1] != D:
+    shape, k_shape = tuple(q.shape), tuple(k.shape)
+    tokens, D = shape[:-2], shape[-1]
+    if k_shape[:-2] != tokens or k_shape[-1] != D:
         raise ValueError("k must have q's tokens and head dimension")
     if not isinstance(inv_freq, _Tensor) or inv_freq.dim() != 1:
         raise ValueError("inv_freq must be a tensor of one frequency for each rotated pair")
     pairs = inv_freq.shape[0]
     args = (_plain(q_weight, "q_weight", dtype, (D,), index), _plain(k_weight, "k_weight", dtype, (D,), index),
-            _plain(positions, "positions", torch.int32, shape[:-2], index),
-            _plain(inv_freq, "inv_freq", torch.float32, (pairs,), index), _DTYPES[dtype],
-            shape[0] if len(shape) == 4 else 1, shape[-3], Hq, k_shape[-2], D, 2 * pairs, 1 if interleaved else 0, eps)
+            _plain(positions, "positions", torch.int32, tokens, index),
+            _plain(inv_freq, "inv_freq", torch.float32, (pairs,), index), code,
+            tokens[0] if len(tokens) == 2 else 1, tokens[-1], shape[-2], k_shape[-2], D, 2 * pairs,
+            1 if interleaved else 0, eps)
     return index, rq, rk, args
 
 
@@ -274,10 +285,12 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interl
     if out is None:
         q_out = torch.empty_like(q, memory_format=_contiguous)
         k_out = torch.empty_like(k, memory_format=_contiguous)
+        ro, rp = _new_rows(q_out), _new_rows(k_out)
     else:
         q_out, k_out = out
-    _call(lib.load().kcg_qk_norm_rope, index, rq, rk, _rows(q_out, "out[0]", q.dtype, index, q.shape),
-          _rows(k_out, "out[1]", q.dtype, index, k.shape), *args)
+        ro = _rows(q_out, "out[0]", q.dtype, index, q.shape)
+        rp = _rows(k_out, "out[1]", q.dtype, index, k.shape)
+    _call(lib.load().kcg_qk_norm_rope, index, rq, rk, ro, rp, *args)
     return q_out, k_out
 
 
@@ -295,9 +308,9 @@ def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, positions, inv_freq,
     gq, gk = torch.empty_like(q, memory_format=_contiguous), torch.empty_like(k, memory_format=_contiguous)
     gwq, gwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
     # (a shape that has no workspace is one that the call refuses)
-    address, size, held = _workspace(workspace, L.kcg_qk_norm_rope_backward_ws_bytes(*args[5:10]) or 16, index)
-    _call(L.kcg_qk_norm_rope_backward, index, rdq, rdk, rq, rk, _rows(gq, "grad_q", dtype, index),
-          _rows(gk, "grad_k", dtype, index), args[0], args[1], gwq.data_ptr(), gwk.data_ptr(), *args[2:], address, size)
+    address, size, held = _workspace(workspace, L.kcg_qk_norm_rope_backward_ws_bytes(*args[5:10]) or 16, index, q.device)
+    _call(L.kcg_qk_norm_rope_backward, index, rdq, rdk, rq, rk, _new_rows(gq), _new_rows(gk), args[0], args[1],
+          gwq.data_ptr(), gwk.data_ptr(), *args[2:], address, size)
     return gq, gk, gwq, gwk
 
 
@@ -323,7 +336,7 @@ class KvCache:
         elif k_exp is not None or v_exp is not None:
             raise ValueError("a bfloat16 cache has no exponents")
         self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
-        self.index = k.get_device()
+        self.index, self.device = k.get_device(), k.device
         pages, self.heads, self.page_size, self.dim = k.shape
         eight = k.dtype == torch.float8_e4m3fn
         if max(k.shape) > 0x7fffffff:
@@ -381,15 +394,16 @@ def kv_cache_read(cache, slots, out_dtype=torch.bfloat16, out=None):
     if out is None:
         if out_dtype not in _DTYPES:
             raise ValueError("a cache is read as float32 or bfloat16")
-        k = torch.empty(shape, dtype=out_dtype, device=cache.k.device)
+        k = torch.empty(shape, dtype=out_dtype, device=cache.device)
         v = torch.empty_like(k)
+        rk, rv = _new_rows(k), _new_rows(v)
     else:
         k, v = out
         out_dtype = k.dtype if isinstance(k, _Tensor) else None
         if out_dtype not in _DTYPES:
             raise ValueError("a cache is read as float32 or bfloat16")
-    _call(lib.load().kcg_kv_cache_read, index, cache._c, at, _rows(k, "out[0]", out_dtype, index, shape),
-          _rows(v, "out[1]", out_dtype, index, shape), _DTYPES[out_dtype], B, S)
+        rk, rv = _rows(k, "out[0]", out_dtype, index, shape), _rows(v, "out[1]", out_dtype, index, shape)
+    _call(lib.load().kcg_kv_cache_read, index, cache._c, at, rk, rv, _DTYPES[out_dtype], B, S)
     return k, v
 
 
@@ -426,15 +440,15 @@ def fmha_cache(q, cache, block_table, context_lens, draft_lens=None, tree_mask=N
     tree = None if tree_mask is None else _plain(tree_mask, "tree_mask", torch.int64, (B, N), index)
     if out is None:
         out_dtype = out_dtype or torch.bfloat16
-        out = (torch.empty if draft_lens is None else torch.zeros)(shape, dtype=out_dtype, device=q.device)
+        out = (torch.empty if draft_lens is None else torch.zeros)(shape, dtype=out_dtype, device=cache.device)
     elif not isinstance(out, _Tensor) or out_dtype not in (None, out.dtype):
         raise ValueError("out must be a tensor of dtype out_dtype")
     out_dtype = out.dtype
     if out_dtype not in _DTYPES:
         raise ValueError("attention over a cache writes bfloat16 or float32, not %s" % out_dtype)
     L = lib.load()
-    address, size, held = _workspace(workspace, workspace is None and L.kcg_fmha_cache_ws_bytes(cache._c, width, B, N, Hq),
-                                     index)
+    need = 0 if workspace is not None else L.kcg_fmha_cache_ws_bytes(cache._c, width, B, N, Hq)
+    address, size, held = _workspace(workspace, need, index, cache.device)
     _call(L.kcg_fmha_cache, index, rq, cache._c, table, width, context, drafts, tree,
           _rows(out, "out", out_dtype, index, shape), _DTYPES[out_dtype], B, N, Hq, scale, address, size)
     return out

@@ -352,7 +352,9 @@ KCG_API int kcg_kv_cache_read(const kcg_kv_cache *cache, const int32_t *slots, c
  * `workspace`: 16-byte aligned device memory that nothing else uses until the call has
  * completed, for partial results where the keys of a sequence are split over several workgroups.
  * kcg_fmha_cache_ws_bytes gives the bytes the preferred split needs (0: none); with fewer, or NULL,
- * the call splits less, down to not at all. */
+ * the call splits less, down to not at all.  Results do not vary between runs of one call; another
+ * workspace size may round differently.  The first launch of a kernel variant on a device raises its
+ * LDS limit (hipFuncSetAttribute). */
 KCG_API int64_t kcg_fmha_cache_ws_bytes(const kcg_kv_cache *cache, int32_t table_width, int32_t B,
                                         int32_t N, int32_t Hq);
 KCG_API int kcg_fmha_cache(const kcg_rows *q, const kcg_kv_cache *cache, const int32_t *block_table,

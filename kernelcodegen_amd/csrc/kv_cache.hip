@@ -3,8 +3,11 @@
 //
 // e4m3 rows share one power of two, 2^(x - 127): a float type loses nothing to a power of two that
 // it would not lose to any other scale (but the one binade at its small end), the scaling of a row
-// is exact, and every dequantised value is a bf16 number.  Both kernels are bound by memory; a row
-// is D / 8 lanes of eight elements, as everywhere.
+// is exact, and every dequantised value is a bf16 number.  A row is D / 8 lanes of eight elements,
+// as everywhere.
+// Reading is bound by memory (32768 tokens, 8 heads of 128, e4m3 to bf16: 33 us, 202 MB, 6.1 TB/s);
+// writing by its instructions and by the comparison of the slots (8191 tokens of the same: 14.5 us for
+// 50 MB, 12.9 without the comparison, where a copy of as much takes 8.5).
 #include "kv_cache.h"
 
 namespace kcg {
@@ -166,7 +169,7 @@ __global__ __launch_bounds__(256) void kv_cache_read_kernel(const KvMoveArgs<T, 
     }
 #pragma unroll
     for (int k = 0; k < ROWS; ++k)
-      if (to[k]) store8<VEC, true>(to[k], x[k]);
+      if (to[k]) store8<VEC, true>(to[k], x[k]);  // (32768 tokens: 48 us through the caches, 35 past them)
   }
 }
 

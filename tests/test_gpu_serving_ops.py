@@ -149,6 +149,32 @@ def test_norm_rope_far_positions_and_strides(dev):
             within(dw, want_w, U * size_w)
 
 
+def test_norm_rope_of_packed_tokens(dev):
+    """[tokens,H,D] is [1,tokens,H,D], also on another stream than the tensors' own."""
+    q, k, wq, wk, pos, freq = (t.to(dev) for t in norm_inputs((1, 37, 4, 2, 64, 32), BF16, 91))
+    dq, dk = torch.randn_like(q), torch.randn_like(k)
+    o = ops()
+    whole = o.qk_norm_rope(q, k, wq, wk, pos, freq) + o.qk_norm_rope_backward(dq, dk, q, k, wq, wk, pos, freq)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        packed = o.qk_norm_rope(q[0], k[0], wq, wk, pos[0], freq) + o.qk_norm_rope_backward(
+            dq[0], dk[0], q[0], k[0], wq, wk, pos[0], freq)
+        torch.cuda.current_stream().synchronize()
+    for a, b in zip(whole, packed):
+        assert b.dim() == min(a.dim(), 3) and torch.equal(a.reshape(b.shape), b)
+
+
+def test_norm_rope_tiny_rows_without_eps(dev):
+    """eps 0 counts as the smallest normal number: rows of zeros give zeros, rows whose squares vanish stay finite."""
+    q, k, wq, wk, pos, freq = norm_inputs((1, 2, 2, 1, 64, 64), F32, 95)
+    q[0, 0] = 0
+    q[0, 1] *= 1e-25
+    got = ops().qk_norm_rope(*(t.to(dev) for t in (q, k, wq, wk, pos, freq)), eps=0.0)
+    for g, x, w in zip(got, (q, k), (wq, wk)):
+        want, size = ref.norm_rope(x, w, pos, freq, torch.finfo(F32).tiny, False)
+        within(g, want, 32 * U * size)
+
+
 def test_norm_rope_in_place_zero_rows_and_nonfinite(dev):
     q, k, wq, wk, pos, freq = norm_inputs((1, 6, 3, 2, 64, 64), BF16, 71)
     q[0, 0, 0] = 0

@@ -323,13 +323,14 @@ typedef struct kcg_kv_cache {
  * slots[B][S].  e4m3: x is the least exponent (at least 1) with which the largest finite magnitude
  * of the row does not exceed 448; values are rounded to nearest, halves to even; infinities and
  * NaN are stored as NaN.  A token whose slot lies outside the cache (-1: padding) is not written;
- * of tokens with the same slot the last one is.  Slots that no token names stay as they were. */
+ * of tokens with the same slot the last one is.  Slots that no token names stay as they were.  The rows
+ * are not parts of the cache. */
 KCG_API int kcg_kv_cache_write(const kcg_kv_cache *cache, const kcg_rows *k, const kcg_rows *v,
                                int dtype, const int32_t *slots, int32_t B, int32_t S,
                                void *stream);
 
 /* The reverse: keys and values of the slots as rows of `dtype`.  A slot outside the cache gives
- * rows of zeros. */
+ * rows of zeros.  The outputs overlap neither the cache nor each other. */
 KCG_API int kcg_kv_cache_read(const kcg_kv_cache *cache, const int32_t *slots, const kcg_rows *k,
                               const kcg_rows *v, int dtype, int32_t B, int32_t S, void *stream);
 
@@ -347,7 +348,8 @@ KCG_API int kcg_kv_cache_read(const kcg_kv_cache *cache, const int32_t *slots, c
  * draft_lens[b] on stay as they were.  Products are bf16 x bf16 in fp32, the softmax fp32; the
  * weights are rounded to bf16 for the second product (fp32 output: split over three bf16 numbers).
  * Lengths below 0 count as 0, draft_lens above N as N; keys beyond the table's last page and keys in
- * pages outside the cache are not seen.
+ * pages outside the cache are not seen.  All tables together may have room for 2^35 keys.  `out` overlaps
+ * nothing that the call reads.
  *
  * `workspace`: 16-byte aligned device memory that nothing else uses until the call has
  * completed, for partial results where the keys of a sequence are split over several workgroups.

@@ -906,6 +906,8 @@ inline int check_fmha_cache(const kcg_kv_cache *cache, int64_t width, int64_t B,
   if (width <= 0 || B <= 0 || N <= 0 || Hq <= 0) return KCG_ERR_BAD_SHAPE;
   if (N > 64 || Hq % cache->heads) return KCG_ERR_UNSUPPORTED_SHAPE;
   if (width > 0x7fffff00LL / cache->page_size || B > 0x7fffffffLL / width) return KCG_ERR_UNSUPPORTED_SHAPE;
+  // (the chunks of all sequences are summed in 32 bits, and lengths may say that every table is full)
+  if (B * width > (int64_t{1} << 35) / cache->page_size) return KCG_ERR_UNSUPPORTED_SHAPE;
   return check_extents(B, N, Hq, cache->dim);
 }
 

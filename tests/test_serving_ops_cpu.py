@@ -117,6 +117,20 @@ def test_fmha_cache_refusals(change, status):
     assert got == status
 
 
+@pytest.mark.parametrize("B, page", [(64, 256), (33, 256), (64, 128), (1024, 64)])
+def test_fmha_cache_refuses_tables_whose_chunks_do_not_count_in_32_bits(B, page):
+    """Units are counted in 32 bits on the device, over whatever lengths it finds: the tables' room bounds them."""
+    L, width = lib.load(), (1 << 35) // page // B
+    c, r = cache(page_size=page), rows()
+
+    def call(width):
+        return L.kcg_fmha_cache(ctypes.byref(r), ctypes.byref(c), P, width, P, None, None, ctypes.byref(rows(h=1)), 1, B,
+                                1, 8, 1.0, None, 0, None)
+    # (the output's rows overlap, so that nothing is launched for what is accepted)
+    assert call(width) == ARGUMENT and L.kcg_fmha_cache_ws_bytes(ctypes.byref(c), width, B, 1, 8) > 0
+    assert call(width + 1) == UNSUPPORTED and L.kcg_fmha_cache_ws_bytes(ctypes.byref(c), width + 1, B, 1, 8) == 0
+
+
 def test_cache_addresses_stay_inside(tmp_path):
     """tests/kv_cache_index_model.cc replays csrc/kv_cache_index.h on the host."""
     exe = str(tmp_path / "model")

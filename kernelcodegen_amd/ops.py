@@ -188,13 +188,14 @@ def fmha(Q, K, V, scale=1.0, causal=False, out=None, out_dtype=None, sched=None)
 # A small call takes as long as its checks: each helper below first asks everything in one
 # expression and looks for what is wrong only where that fails.
 _Tensor, _contiguous, _pack_rows = torch.Tensor, torch.contiguous_format, lib.pack_rows
+_TOO_MANY = 1 << 31  # (extents are 32-bit numbers in the C interface)
 
 
 def _rows(t, name, dtype, index, shape=None):
     """kcg_rows of a [B,S,H,D] (or [tokens,H,D]) tensor on device `index`: any strides but a
     contiguous last axis."""
     if isinstance(t, _Tensor) and t.dtype == dtype and t.get_device() == index and (
-            shape is None or t.shape == shape):
+            shape is None or t.shape == shape) and t.numel() < _TOO_MANY:
         stride = t.stride()
         if len(stride) == 4 and stride[3] == 1:
             return _pack_rows(t.data_ptr(), stride[0], stride[1], stride[2])
@@ -208,6 +209,8 @@ def _rows(t, name, dtype, index, shape=None):
         raise ValueError("%s must have dtype %s, not %s" % (name, dtype, t.dtype))
     if shape is not None and t.shape != shape:
         raise ValueError("%s must have shape %s, not %s" % (name, tuple(shape), tuple(t.shape)))
+    if t.numel() >= _TOO_MANY:
+        raise ValueError("%s must have fewer than 2^31 elements" % name)
     raise ValueError("the last axis of %s must be contiguous" % name)
 
 
@@ -434,6 +437,8 @@ def fmha_cache(q, cache, block_table, context_lens, draft_lens=None, tree_mask=N
     if not isinstance(block_table, _Tensor) or block_table.dim() != 2:
         raise ValueError("block_table must be an int32 tensor [B, pages]")
     width = block_table.shape[1]
+    if width >= _TOO_MANY:
+        raise ValueError("block_table must have fewer than 2^31 pages to a sequence")
     table = _plain(block_table, "block_table", torch.int32, (B, width), index)
     context = _plain(context_lens, "context_lens", torch.int32, (B,), index)
     drafts = None if draft_lens is None else _plain(draft_lens, "draft_lens", torch.int32, (B,), index)

@@ -131,6 +131,25 @@ def test_fmha_cache_refuses_tables_whose_chunks_do_not_count_in_32_bits(B, page)
     assert call(width + 1) == UNSUPPORTED and L.kcg_fmha_cache_ws_bytes(ctypes.byref(c), width + 1, B, 1, 8) == 0
 
 
+def test_extents_beyond_32_bits_are_refused():
+    """The C interface counts tokens and pages in 32 bits: 2^32 + 4 of them must not become 4."""
+    torch = pytest.importorskip("torch")
+    from kernelcodegen_amd import ops
+    many = (1 << 32) + 4
+    # tensors without memory, whose device index is that of the cache
+    handle = ops.KvCache.__new__(ops.KvCache)
+    handle.index, handle.heads, handle.dim, handle._c = -1, 8, 128, cache(k=None)
+    rows = torch.empty(1, 8, 128, dtype=torch.bfloat16, device="meta").expand(many, 8, 128)
+    slots = torch.empty(many, dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.kv_cache_write(handle, rows, rows, slots)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.kv_cache_read(handle, slots, out=(rows, rows))
+    q = torch.empty(1, 1, 8, 128, dtype=torch.bfloat16, device="meta")
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.fmha_cache(q, handle, slots.view(1, many), torch.empty(1, dtype=torch.int32, device="meta"), out=q)
+
+
 def test_cache_addresses_stay_inside(tmp_path):
     """tests/kv_cache_index_model.cc replays csrc/kv_cache_index.h on the host."""
     exe = str(tmp_path / "model")

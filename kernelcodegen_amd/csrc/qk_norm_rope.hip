@@ -33,7 +33,7 @@ struct NormRopeArgs {
 constexpr int kNrWaves = 4;
 
 // cos and sin of the token's angles for this lane's eight elements.  Half pairing: one angle per
-// element; interleaved: one per two elements.  Elements that are not rotated get (1, 0).
+// element; interleaved: one per two elements.  Elements that are not rotated get (1, 0), which is not used.
 template <int D, bool INTERLEAVED, typename T>
 __device__ __forceinline__ void load_turns(const NormRopeArgs<T> &a, int token, float *turns, int lane,
                                            float (&cs)[8], float (&sn)[8]) {
@@ -61,15 +61,17 @@ __device__ __forceinline__ void load_turns(const NormRopeArgs<T> &a, int token, 
   }
 }
 
-// Rotates the row by the angles (cs, sn).
+// Rotates the row by the angles (cs, sn).  Elements behind the rotated ones are left out, not turned by (1, 0),
+// for which an infinity beside one would make it NaN.
 template <int D, bool INTERLEAVED>
 __device__ __forceinline__ void rotate(float (&y)[8], const float (&cs)[8], const float (&sn)[8], int rot, int lane) {
+  const bool rotated = 8 * (lane % (D / 8)) < rot;
   if (INTERLEAVED) {
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
       const float a = y[j], b = y[j + 1];
-      y[j] = a * cs[j] - b * sn[j];
-      y[j + 1] = b * cs[j] + a * sn[j];
+      y[j] = rotated ? a * cs[j] - b * sn[j] : a;
+      y[j + 1] = rotated ? b * cs[j] + a * sn[j] : b;
     }
   } else {
     // the other element of a pair is rot / 2 further on, or back, in lane +- rot / 16
@@ -79,7 +81,8 @@ __device__ __forceinline__ void rotate(float (&y)[8], const float (&cs)[8], cons
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float other = __shfl(y[j], from);
-      y[j] = first ? y[j] * cs[j] - other * sn[j] : y[j] * cs[j] + other * sn[j];
+      const float turned = first ? y[j] * cs[j] - other * sn[j] : y[j] * cs[j] + other * sn[j];
+      y[j] = rotated ? turned : y[j];
     }
   }
 }

@@ -191,6 +191,28 @@ def test_norm_rope_in_place_zero_rows_and_nonfinite(dev):
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_norm_rope_infinity_behind_the_rotated_elements(dev, interleaved):
+    """An element that is not rotated mixes with no other: beside an infinity the formula's zeros stay zeros,
+    and the gradients of other weights stay numbers."""
+    q, k, wq, wk, pos, freq = norm_inputs((1, 3, 2, 1, 64, 32), F32, 97)
+    dq, dk = normal(98, *q.shape), normal(99, *k.shape)
+    at = 41
+    q[0, 1, 1, at] = math.inf
+    args = [t.to(dev) for t in (q, k, wq, wk, pos, freq)]
+    got = ops().qk_norm_rope(*args, interleaved=interleaved)[0].cpu()
+    want, _ = ref.norm_rope(q, wq, pos, freq, 1e-6, interleaved)
+    assert want.isnan().sum() == 1 and torch.equal(got.isnan(), want.isnan())
+    assert (got[0, 1, 1].nan_to_num() == 0).all()
+    q[0, 1, 1, at], dq[0, 1, 1, at] = 1.0, math.inf
+    args[0] = q.to(dev)
+    dw = ops().qk_norm_rope_backward(dq.to(dev), dk.to(dev), *args, interleaved=interleaved)[2].cpu()
+    _, want, _, bound = ref.norm_rope_backward(dq, q, wq, pos, freq, 1e-6, interleaved)
+    rest = torch.arange(64) != at
+    assert want[rest].isfinite().all() and want[at].isinf() and dw[at] == want[at]
+    within(dw[rest], want[rest], U * bound[rest])
+
+
 def test_norm_rope_backward_repeats_bit_for_bit(dev):
     q, k, wq, wk, pos, freq = (t.to(dev) for t in norm_inputs((2, 700, 6, 2, 128, 128), BF16, 81))
     dq, dk = torch.randn_like(q), torch.randn_like(k)

@@ -542,12 +542,23 @@ __global__ __launch_bounds__(64 * kFcWaves, QT == 1 && (D == 64 || TERMS == 1) ?
             for (int k = 0; k < 2; ++k)
               y[k] = __builtin_ldexpf(y[k], static_cast<int>(x[w2 / 2] << (24 - 8 * (2 * (w2 % 2) + k))) >> 24);
           }
+          if constexpr (TERMS == 1) {
+            p[t][kb][0][w2] = float_to_bf16_pair(y[0], y[1]);
+          } else {
+            // Terms cut off after eight bits each, which hold all 24 of a weight.  None of a weight's is negative, or,
+            // against values that may be infinite (e4m3 has no infinity), zero: those would make NaN of an infinity.
+            const float least[2] = {E8 ? 0.0f : y[0] * 0x1p-30f, E8 ? 0.0f : y[1] * 0x1p-30f};
 #pragma unroll
-          for (int z = 0; z < TERMS; ++z) {
-            const unsigned pair = float_to_bf16_pair(y[0], y[1]);
-            p[t][kb][z][w2] = pair;
-            y[0] -= __builtin_bit_cast(float, pair << 16);
-            y[1] -= __builtin_bit_cast(float, pair & 0xffff0000u);
+            for (int z = 0; z < TERMS; ++z) {
+              if (!E8 && z) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) y[k] = fmaxf(y[k], least[k]);
+              }
+              const unsigned a = __builtin_bit_cast(unsigned, y[0]), b = __builtin_bit_cast(unsigned, y[1]);
+              p[t][kb][z][w2] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+              y[0] -= __builtin_bit_cast(float, a & 0xffff0000u);
+              y[1] -= __builtin_bit_cast(float, b & 0xffff0000u);
+            }
           }
         }
     };

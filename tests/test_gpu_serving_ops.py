@@ -513,6 +513,35 @@ def test_fmha_cache_one_value_not_finite(dev, kind):
     assert torch.equal(torch.isfinite(out), finite)
 
 
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("context, N, D", [(200, 1, 64), (200, 9, 128), (1500, 2, 128)])
+def test_fmha_cache_values_of_infinity(dev, context, N, D, out_dtype):
+    """Weights are positive: an infinity among the values that every query sees is the output of its column, infinities
+    of both signs in a column give NaN, and the other columns are what they are without them."""
+    page, width = 16, 100
+    cache = filled_cache(dev, width, 2, page, D, BF16)
+    table = make_table(1, width, width, 3)
+    clean = cache_values(cache)
+
+    def put(key, column, value):
+        cache.v[int(table[0, key // page]), :, key % page, column] = value
+    put(5, 7, math.inf)
+    put(40, 9, -math.inf)
+    put(33, 11, math.inf)
+    put(150, 11, -math.inf)
+    put(context - 1, 50, math.inf)  # in a chunk that reaches beyond the context
+    q = normal(1, 1, N, 8, D, dtype=BF16)
+    got = ops().fmha_cache(q.to(dev), cache, table.to(dev), torch.tensor([context], dtype=torch.int32, device=dev), scale=0.1,
+                           out_dtype=out_dtype).cpu()
+    want, arith, weight = ref.fmha_cache(q, *clean, table, [context], None, None, 0.1, torch.zeros(q.shape))
+    assert (got[..., 7] == math.inf).all() and (got[..., 9] == -math.inf).all() and (got[..., 50] == math.inf).all()
+    assert got[..., 11].isnan().all()
+    rest = torch.ones(D, dtype=torch.bool)
+    rest[[7, 9, 11, 50]] = False
+    off = 2.0 ** -24 if out_dtype == F32 else 2.0 ** -8  # as in check_fmha
+    within(got[..., rest], want[..., rest], (arith + off * (1 + 4 * off) * weight)[..., rest])
+
+
 def test_fmha_cache_large_scores(dev):
     """Scores far apart and rising along the keys: the running maximum moves in every tile."""
     cache = filled_cache(dev, 40, 1, 16, 64, BF16)

@@ -149,7 +149,7 @@ inline int check_rows(const kcg_rows *r, int dtype, int B, int S, int H, int D, 
         if (extent[i] > 1 && (least < 0 || stride[i] < stride[least])) least = i;
       if (least < 0) break;
       if (stride[least] < below) return KCG_ERR_BAD_ARGUMENT;
-      if (stride[least] > (int64_t{1} << 48)) return KCG_ERR_BAD_ARGUMENT;
+      if (stride[least] > (int64_t{1} << 48) / (extent[least] - 1)) return KCG_ERR_BAD_ARGUMENT;  // (more than any memory)
       below += stride[least] * (extent[least] - 1);
       extent[least] = 1;
     }

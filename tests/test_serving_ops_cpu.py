@@ -48,6 +48,13 @@ def test_norm_rope_refusals(change, status):
     assert norm_rope(**change) == status
 
 
+def test_rows_beyond_any_memory_are_refused():
+    """2^48 elements times 2^16 steps do not count as none: rows of two heads would be the same."""
+    far = rows(s=1 << 48, h=1 << 48)
+    assert norm_rope(qo=far, S=65537, Hq=2, Hk=1) == ARGUMENT
+    assert norm_rope(ko=far, S=65537, Hq=1, Hk=2) == ARGUMENT
+
+
 def test_norm_rope_backward_refusals():
     L = lib.load()
     need = L.kcg_qk_norm_rope_backward_ws_bytes(1, 4, 8, 8, 128)

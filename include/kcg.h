@@ -283,7 +283,8 @@ typedef struct kcg_rows {
  * `dtype` (KCG_F32 or KCG_BF16).  Arithmetic is fp32 (angles: 64 bits), one rounding at the end.
  * D is 64 or 128; rot_dim a multiple of 16 from 16 to D; eps 0 or more (below the smallest normal number it
  * counts as that).  An output may be its own input (same data and strides); otherwise outputs
- * overlap no input and not each other. */
+ * overlap no input and not each other (two outputs that begin at one address: KCG_ERR_BAD_ARGUMENT, as in
+ * the two calls below that have several). */
 KCG_API int kcg_qk_norm_rope(const kcg_rows *q, const kcg_rows *k, const kcg_rows *q_out,
                              const kcg_rows *k_out, const void *q_weight, const void *k_weight,
                              const int32_t *positions, const float *inv_freq, int dtype, int32_t B,

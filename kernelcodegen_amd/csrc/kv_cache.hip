@@ -229,6 +229,7 @@ int check_and_move(const kcg_kv_cache *cache, const kcg_rows *k, const kcg_rows 
   if (const int e = check_extents(B, S, cache->heads, cache->dim)) return e;
   if (const int e = check_rows(k, dtype, B, S, cache->heads, cache->dim, !WRITE)) return e;
   if (const int e = check_rows(v, dtype, B, S, cache->heads, cache->dim, !WRITE)) return e;
+  if (!WRITE && k->data == v->data) return KCG_ERR_BAD_ARGUMENT;
   if (dtype == KCG_F32)
     return cache->dtype == KCG_E4M3 ? move<WRITE, float, uint8_t>(*cache, *k, *v, dtype, slots, B, S, stream)
                                     : move<WRITE, float, uint16_t>(*cache, *k, *v, dtype, slots, B, S, stream);

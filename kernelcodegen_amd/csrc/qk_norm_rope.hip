@@ -346,6 +346,7 @@ int kcg_qk_norm_rope(const kcg_rows *q, const kcg_rows *k, const kcg_rows *q_out
   if (const int e = kcg::check_rows(k, dtype, B, S, Hk, D, false)) return e;
   if (const int e = kcg::check_rows(q_out, dtype, B, S, Hq, D, true)) return e;
   if (const int e = kcg::check_rows(k_out, dtype, B, S, Hk, D, true)) return e;
+  if (q_out->data == k_out->data) return KCG_ERR_BAD_ARGUMENT;
   hipStream_t st = static_cast<hipStream_t>(stream);
   return dtype == KCG_F32
              ? kcg::norm_rope<float>(q, k, nullptr, nullptr, q_out, k_out, q_weight, k_weight, nullptr, nullptr,
@@ -379,7 +380,8 @@ int kcg_qk_norm_rope_backward(const kcg_rows *dq, const kcg_rows *dk, const kcg_
   if (!grad_q_weight || !grad_k_weight || !workspace) return KCG_ERR_NULL_POINTER;
   if (reinterpret_cast<uintptr_t>(grad_q_weight) % kcg::element_bytes(dtype) ||
       reinterpret_cast<uintptr_t>(grad_k_weight) % kcg::element_bytes(dtype) || !kcg::aligned16(workspace) ||
-      workspace_bytes < kcg_qk_norm_rope_backward_ws_bytes(B, S, Hq, Hk, D))
+      workspace_bytes < kcg_qk_norm_rope_backward_ws_bytes(B, S, Hq, Hk, D) || grad_q->data == grad_k->data ||
+      grad_q_weight == grad_k_weight)
     return KCG_ERR_BAD_ARGUMENT;
   hipStream_t st = static_cast<hipStream_t>(stream);
   return dtype == KCG_F32

@@ -105,6 +105,19 @@ def test_cache_row_refusals():
     assert L.kcg_kv_cache_read(c, P, r, none, 1, 1, 4, None) == NULL
 
 
+def test_one_memory_for_two_outputs_is_refused():
+    """Which of the two rows it held in the end would be a matter of chance."""
+    L = lib.load()
+    assert norm_rope(qo=rows(2 * P), ko=rows(2 * P)) == ARGUMENT
+    r, other = ctypes.byref(rows()), ctypes.byref(rows(2 * P))
+
+    def backward(gq, gwq):
+        return L.kcg_qk_norm_rope_backward(r, r, r, r, gq, r, P, P, gwq, P, P, P, 1, 1, 4, 8, 8, 128, 128, 0, 1e-6, P,
+                                           1 << 30, None)
+    assert backward(r, 2 * P) == ARGUMENT and backward(other, P) == ARGUMENT
+    assert L.kcg_kv_cache_read(ctypes.byref(cache()), P, other, other, 1, 1, 4, None) == ARGUMENT
+
+
 @pytest.mark.parametrize("change, status", [
     (dict(table=None), NULL), (dict(context=None), NULL), (dict(q=rows(None)), NULL), (dict(out=rows(None)), NULL),
     (dict(o_dtype=2), ARGUMENT), (dict(scale=float("nan")), ARGUMENT), (dict(scale=float("inf")), ARGUMENT),

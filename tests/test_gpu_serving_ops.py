@@ -572,6 +572,47 @@ def test_fmha_cache_many_sequences(dev, B, longest):
         check_fmha(dev, cache, q, table, context.tolist(), drafts.tolist(), None, 0.125, F32, workspace=workspace)
 
 
+def marked_workspace(cache, table, N, Hq, size=None):
+    """A workspace of the preferred (or the given) size whose bytes show whether partial results were stored."""
+    B, width = table.shape
+    need = ops().fmha_cache_workspace_bytes(cache, width, B, N, Hq)
+    assert need > 0
+    return torch.full((need if size is None else size,), 0xa5, dtype=torch.uint8, device=cache.device)
+
+
+def was_cut(workspace, cache):
+    """The first row of the first slot is stored if any sequence was cut."""
+    return bool((workspace[:4 * cache.dim] != 0xa5).any())
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("B, longest", [(65, 900), (130, 700), (1024, 500), (1100, 1000), (2100, 600)])
+def test_fmha_cache_many_sequences_of_which_some_are_cut(dev, B, longest, out_dtype):
+    """More sequences than lanes, and more than one pass of the launch that finds their units takes: the long ones, on
+    both sides of a pass's end, are cut and joined, among empty ones, short ones and ones without drafts."""
+    N, Hq, Hk, D, page = 2, 2, 1, 64, 16
+    g = gen(B)
+    context = torch.randint(0, 40, (B,), generator=g)
+    context[::9] = 0
+    drafts = torch.randint(0, N + 1, (B,), generator=g)
+    far = [b for b in (3, 64, 999, 1022, 1023, 1024, 1025, 1099, 2047, 2048, 2099) if b < B] + [B - 1]
+    for i, b in enumerate(far):
+        context[b], drafts[b] = longest - 37 * i, N
+    context[5], drafts[5] = longest, 0
+    width = 60  # more room than any of them needs
+    cache = filled_cache(dev, 90, Hk, page, D, BF16)
+    table = torch.randint(0, 90, (B, width), generator=g).to(torch.int32)
+    q = normal(1, B, N, Hq, D, dtype=BF16)
+    need = ops().fmha_cache_workspace_bytes(cache, width, B, N, Hq)
+    got = []
+    for size in (need, need, need // 3):
+        workspace = marked_workspace(cache, table, N, Hq, size)
+        got.append(check_fmha(dev, cache, q, table, context.tolist(), drafts.tolist(), None, 0.125, out_dtype,
+                              workspace=workspace))
+        assert was_cut(workspace, cache)
+    assert torch.equal(got[0], got[1])
+
+
 def test_fmha_cache_no_queries_at_all(dev):
     for B in (3, 100):
         cache = filled_cache(dev, 64, 2, 16, 128, E4M3)

@@ -658,6 +658,56 @@ def test_fmha_cache_query_layouts(dev):
         within(ops().fmha_cache(fused[:, :, :Hq], *args, scale=0.1, workspace=ws), exact, arith + 2.0 ** -8 * 1.02 * weight)
 
 
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", [BF16, E4M3])
+def test_fmha_cache_layouts_and_workspaces_of_cut_sequences(dev, kind, out_dtype):
+    """Outputs in every layout through the joining launch; smaller workspaces split less, down to not at all."""
+    B, N, Hq, Hk, D, page = 2, 3, 6, 2, 128, 16
+    cache = filled_cache(dev, 200, Hk, page, D, kind)
+    table, context = make_table(B, 100, 200, 1), [1500, 903]
+    fused = normal(1, B, N, Hq + 4, D, dtype=BF16).to(dev)
+    q = fused[:, :, :Hq]
+    workspace = marked_workspace(cache, table, N, Hq)
+    want = check_fmha(dev, cache, q.cpu(), table, context, None, None, 0.1, out_dtype, workspace=workspace)
+    assert was_cut(workspace, cache)
+    args = (cache, table.to(dev), torch.tensor(context, dtype=torch.int32, device=dev))
+    assert torch.equal(ops().fmha_cache(q, *args, scale=0.1, out_dtype=out_dtype), want)  # its own workspace
+    odd = torch.zeros(B * N * Hq * (D + 1) + 1, dtype=BF16, device=dev)[1:].view(B, N, Hq, D + 1)[..., :D].copy_(q)
+    outs = (torch.empty(B, Hq, N, D, dtype=out_dtype, device=dev).transpose(1, 2),
+            torch.empty(B, N, Hq, D + 1, dtype=out_dtype, device=dev)[..., 1:],
+            torch.empty(N, B, Hq + 1, D, dtype=out_dtype, device=dev).transpose(0, 1)[:, :, 1:])
+    for x in (q, odd):
+        for out in outs:
+            out.fill_(-1)
+            assert torch.equal(ops().fmha_cache(x, *args, scale=0.1, out=out), want)
+    need = workspace.numel()
+    cut = []
+    for size in (0, 16, need // 16, need // 8, need - 1, need + 100):
+        workspace = marked_workspace(cache, table, N, Hq, size)
+        check_fmha(dev, cache, q.cpu(), table, context, None, None, 0.1, out_dtype, workspace=workspace)
+        cut.append(was_cut(workspace, cache))
+    assert cut[:2] == [False, False] and cut[2:] == [True] * 4
+
+
+@pytest.mark.parametrize("kind", [BF16, E4M3])
+def test_fmha_cache_large_scores_across_units(dev, kind):
+    """Scores that rise (or fall) along keys which several workgroups share: the units' maxima are far apart."""
+    page, pages = 16, 60
+    cache = filled_cache(dev, pages, 1, page, 64, kind)
+    table = torch.arange(pages, dtype=torch.int32).view(1, pages)
+    ramp = torch.linspace(-1, 1, pages * page).view(pages, 1, page, 1)
+    q = normal(1, 1, 2, 8, 64, dtype=BF16).abs()
+    slots = torch.arange(pages * page, dtype=torch.int32, device=dev)
+    v = normal(2, pages * page, 1, 64, dtype=BF16).to(dev)
+    for sign in (1, -1):
+        k = (sign * ramp * torch.ones(64) * 8).to(BF16).reshape(-1, 1, 64).to(dev)
+        ops().kv_cache_write(cache, k, v, slots)
+        for scale in (1.0, 30.0):
+            workspace = marked_workspace(cache, table, 2, 8)
+            check_fmha(dev, cache, q, table, [957], None, None, scale, F32, workspace=workspace)
+            assert was_cut(workspace, cache)
+
+
 def test_cache_beyond_32_bits(dev):
     """A cache of 2^32 elements and more: its last pages are written, read and attended to."""
     heads, page, dim = 8, 256, 128
@@ -808,6 +858,56 @@ def test_captured_steps_replay(dev):
         assert torch.equal(outs[0], eager)
         for a, b in zip(grads, back()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("B", [3, 70])
+def test_captured_attention_of_cut_sequences_replays(dev, B):
+    """Two captured calls with the launches that find units and join them, in workspaces of the capture's own,
+    replayed with eager work between and with lengths, tables and keys that change."""
+    o = ops()
+    N, Hq, Hk, D, page, width = 2, 8, 2, 64, 16, 64
+    cache = filled_cache(dev, 100, Hk, page, D, BF16)
+    q = normal(1, B, N, Hq, D, dtype=BF16).to(dev)
+    table = torch.randint(0, 100, (B, width), generator=gen(2)).to(torch.int32).to(dev)
+    context = torch.full((B,), 900, dtype=torch.int32, device=dev)
+    drafts = torch.full((B,), N, dtype=torch.int32, device=dev)
+    assert o.fmha_cache_workspace_bytes(cache, width, B, N, Hq) > 0
+    outs = [torch.zeros(B, N, Hq, D, dtype=t, device=dev) for t in (BF16, F32)]
+
+    def call(out):
+        return o.fmha_cache(q, cache, table, context, draft_lens=drafts, scale=0.125, out=out)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for out in outs:
+            call(out)
+    side.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in outs]
+    for graph, out in zip(graphs, outs):
+        with torch.cuda.graph(graph):
+            call(out)
+    g = gen(3)
+    for round_ in range(4):
+        q.copy_(normal(10 + round_, *q.shape, dtype=BF16))
+        cache.k.copy_(normal(20 + round_, *cache.k.shape, dtype=BF16))
+        lengths = torch.randint(0, 60, (B,), generator=g).to(torch.int32)
+        lengths[round_ % B], lengths[-1] = 1000 - 100 * round_, 1022
+        context.copy_(lengths)
+        drafts.copy_(torch.randint(0, N + 1, (B,), generator=g).to(torch.int32))
+        drafts[-1] = N
+        table.copy_(torch.randint(0, 100, (B, width), generator=g).to(torch.int32))
+        for out in outs:
+            out.fill_(-1)
+        for graph in graphs + graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for out in outs:
+            assert torch.equal(out, call(torch.full_like(out, -1)))
+        workspace = marked_workspace(cache, table, N, Hq)
+        got = check_fmha(dev, cache, q.cpu(), table.cpu(), lengths.tolist(), drafts.tolist(), None, 0.125, F32,
+                         workspace=workspace)
+        assert was_cut(workspace, cache)
+        live = (torch.arange(N, device=dev) < drafts[:, None])[..., None, None]
+        assert torch.equal(torch.where(live, got, -1.0), outs[1])
 
 
 def test_two_streams_at_once(dev):

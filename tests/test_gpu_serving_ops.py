@@ -213,6 +213,27 @@ def test_norm_rope_infinity_behind_the_rotated_elements(dev, interleaved):
     within(dw[rest], want[rest], U * bound[rest])
 
 
+@pytest.mark.parametrize("dtype, tokens", [(BF16, 16384), (F32, 8192)])
+def test_norm_rope_outputs_past_the_caches(dev, dtype, tokens):
+    """Outputs of 256 MiB and more are stored past the caches: the same bits as in parts, and the definition's values."""
+    hq, hk, d = 48, 16, 128
+    assert tokens * (hq + hk) * d * dtype.itemsize >= 1 << 28
+    g = torch.Generator(device=dev).manual_seed(5)
+    q, k = (torch.randn(1, tokens, h, d, generator=g, device=dev, dtype=dtype) for h in (hq, hk))
+    wq, wk = (1 + 0.3 * torch.randn(2, d, generator=g, device=dev)).to(dtype)
+    pos = torch.randint(0, 100, (1, tokens), generator=g, device=dev, dtype=torch.int32)
+    freq = (1e4 ** (-torch.arange(64, dtype=torch.float64) / 64)).float().to(dev)
+    got = ops().qk_norm_rope(q, k, wq, wk, pos, freq)
+    cut = tokens // 2 - 1
+    parts = [ops().qk_norm_rope(q[:, at], k[:, at], wq, wk, pos[:, at], freq) for at in (slice(0, cut), slice(cut, None))]
+    for i, g in enumerate(got):
+        assert torch.equal(g, torch.cat([p[i] for p in parts], 1))
+    some = torch.tensor([0, 1, cut, tokens - 2, tokens - 1])
+    for g, x, w in zip(got, (q, k), (wq, wk)):
+        want, size = ref.norm_rope(x[:, some].cpu(), w.cpu(), pos[:, some].cpu(), freq.cpu(), 1e-6, False)
+        within(g[:, some], want, 32 * U * size)  # as in test_norm_rope
+
+
 def test_norm_rope_backward_repeats_bit_for_bit(dev):
     q, k, wq, wk, pos, freq = (t.to(dev) for t in norm_inputs((2, 700, 6, 2, 128, 128), BF16, 81))
     dq, dk = torch.randn_like(q), torch.randn_like(k)
@@ -344,6 +365,26 @@ def test_cache_write_same_slot_twice(dev, tokens):
     slots[tokens // 3] = 2 ** 31 - 1
     want = expected_write(cache, k, v, slots)
     for _ in range(3):
+        ops().kv_cache_write(cache, k.to(dev), v.to(dev), slots.to(dev))
+        assert_cache_holds(cache, want)
+
+
+@pytest.mark.parametrize("kind", [E4M3, BF16])
+@pytest.mark.parametrize("tokens, heads, dim", [(6500, 2, 64), (8192 + 300, 1, 128), (2 * 8192 + 1, 2, 64)])
+def test_cache_write_of_long_prompts(dev, tokens, heads, dim, kind):
+    """Four tokens to a workgroup, and calls that are cut into launches of 8192 tokens: slots named twice inside a
+    workgroup, inside a launch, and in two launches hold the last token."""
+    cache = filled_cache(dev, 500, heads, 16, dim, kind)
+    k, v = normal(1, tokens, heads, dim, dtype=BF16), normal(2, tokens, heads, dim, dtype=BF16)
+    slots = torch.randint(-3, 8003, (tokens,), generator=gen(3)).to(torch.int32)
+    slots[1::50] = slots[0::50][:slots[1::50].numel()]  # neighbours
+    slots[-1] = slots[0]
+    if tokens > 8192:
+        slots[8191], slots[8192] = 77, 77  # on both sides of a launch's end
+        late = slots[8192:]
+        assert torch.isin(slots[:8192], late[late >= 0]).any()
+    want = expected_write(cache, k, v, slots)
+    for _ in range(2):
         ops().kv_cache_write(cache, k.to(dev), v.to(dev), slots.to(dev))
         assert_cache_holds(cache, want)
 
@@ -611,6 +652,41 @@ def test_fmha_cache_many_sequences_of_which_some_are_cut(dev, B, longest, out_dt
                               workspace=workspace))
         assert was_cut(workspace, cache)
     assert torch.equal(got[0], got[1])
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", [BF16, E4M3])
+@pytest.mark.parametrize("B, N, Hq, Hk, D", [(24, 3, 8, 8, 64), (64, 1, 8, 8, 128), (9, 5, 24, 8, 128)])
+def test_fmha_cache_cut_batches(dev, B, N, Hq, Hk, D, kind, out_dtype):
+    """Batches of up to 64 sequences that are not few for the chip: every wave finds its unit, and a joining workgroup
+    takes several rows, the last one fewer."""
+    page, width = 16, 80
+    context = [37 * (b * 7 % B) * 32 // B % 1250 for b in range(B)]
+    context[1], context[B - 1] = 1250, 0
+    drafts = [max(0, N - b % 4) for b in range(B)] if N > 1 else [b % 5 and 1 for b in range(B)]
+    drafts[1] = N
+    cache = filled_cache(dev, 200, Hk, page, D, kind, seed=B)
+    table = torch.randint(0, 200, (B, width), generator=gen(B)).to(torch.int32)
+    q = normal(7, B, N, Hq, D, dtype=BF16)
+    workspace = marked_workspace(cache, table, N, Hq)
+    check_fmha(dev, cache, q, table, context, drafts, random_trees(B, N, 9), D ** -0.5, out_dtype, workspace=workspace)
+    assert was_cut(workspace, cache)
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", [BF16, E4M3])
+@pytest.mark.parametrize("N, Hq, D", [(1, 8, 128), (9, 16, 128), (1, 8, 64), (20, 16, 64)])
+def test_fmha_cache_tables_with_room_beyond_the_caches(dev, N, Hq, D, kind, out_dtype):
+    """Keys and values are requested past the caches where all tables together have room for more than 192 MiB."""
+    B, Hk, page = 3, 8, 16
+    width = (192 << 20) // (B * page * Hk * D * 2 * kind.itemsize) + 1
+    cache = filled_cache(dev, 70, Hk, page, D, kind, seed=N)
+    table = torch.randint(0, 70, (B, width), generator=gen(N)).to(torch.int32)
+    q = normal(7, B, N, Hq, D, dtype=BF16)
+    workspace = marked_workspace(cache, table, N, Hq)
+    for context in ([700, 15, 1201], [33, 0, 64]):
+        check_fmha(dev, cache, q, table, context, None, None, D ** -0.5, out_dtype, workspace=workspace)
+    assert was_cut(workspace, cache)
 
 
 def test_fmha_cache_no_queries_at_all(dev):

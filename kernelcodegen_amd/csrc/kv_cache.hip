@@ -131,8 +131,8 @@ __global__ __launch_bounds__(256) void kv_cache_write_kernel(const KvMoveArgs<co
   }
 }
 
-// `group` tokens to a workgroup; up to ROWS rows of a lane are on their way at a time.
-template <typename T, typename C, int D, bool VEC, int ROWS>
+// `group` tokens to a workgroup; up to ROWS rows of a lane are on their way at a time.  STREAM: outputs past the caches.
+template <typename T, typename C, int D, bool VEC, int ROWS, bool STREAM>
 __global__ __launch_bounds__(256) void kv_cache_read_kernel(const KvMoveArgs<T, C> a, int group) {
   constexpr int LANES = D / 8, PER = 256 / LANES;
   const int lane = threadIdx.x % LANES;
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(256) void kv_cache_read_kernel(const KvMoveArgs<T, 
     }
 #pragma unroll
     for (int k = 0; k < ROWS; ++k)
-      if (to[k]) store8<VEC, true>(to[k], x[k]);  // (32768 tokens: 48 us through the caches, 35 past them)
+      if (to[k]) store8<VEC, STREAM>(to[k], x[k]);
   }
 }
 
@@ -196,10 +196,18 @@ int run_write(const KvMoveArgs<const T, C> &a, hipStream_t stream) {
 template <typename T, typename C, int D, bool VEC>
 int run_read(const KvMoveArgs<T, C> &a, hipStream_t stream) {
   const int per = 256 / (D / 8), rows = 2 * a.cache.shape.heads;
-  // two rows to a lane (32768 tokens, 8 heads of 128, e4m3 to bf16: 54 us with one, 47 with two or four)
+  // two rows to a lane (8 heads of 128, e4m3 to bf16: 32768 tokens 39.0 us with one, 35.7 with two, 34.5 with four; 512
+  // tokens 3.0, 3.4 and 4.3)
   int group = 2 * per / rows;
   if (group < 1) group = 1;
-  return launch(kv_cache_read_kernel<T, C, D, VEC, 2>, dim3((a.tokens + group - 1) / group), dim3(256), 0, stream, a, group);
+  const dim3 grid((a.tokens + group - 1) / group);
+  // Outputs that the L2s hold (4 MiB on each of 8 XCDs) are left in them for the attention that reads them next: 1000
+  // tokens and it take 36 us so, 41 past the caches, 8192 tokens (32 MiB) 178 and 212, alone 12.5 and 11.1.  With more
+  // the two together take the same either way (12288 tokens: 365 and 362, 32768: 1873 and 1878), and the read alone
+  // 29 and 20 with 16384, 52 and 35 with 32768.
+  if (VEC && static_cast<int64_t>(a.tokens) * rows * D * static_cast<int64_t>(sizeof(T)) > int64_t{32} << 20)
+    return launch(kv_cache_read_kernel<T, C, D, VEC, 2, VEC>, grid, dim3(256), 0, stream, a, group);
+  return launch(kv_cache_read_kernel<T, C, D, VEC, 2, false>, grid, dim3(256), 0, stream, a, group);
 }
 
 template <bool WRITE, typename T, typename C>

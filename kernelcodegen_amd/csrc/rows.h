@@ -66,7 +66,7 @@ __device__ __forceinline__ void load8(const uint16_t *p, float (&x)[8]) {
     for (int j = 0; j < 8; ++j) x[j] = bf16_to_float(p[j]);
   }
 }
-// STREAM: past the caches, for outputs larger than them that nothing reads at once
+// STREAM: past the caches, for outputs larger than those that would serve their reader
 template <bool STREAM, typename V>
 __device__ __forceinline__ void store_vector(V x, void *p) {
   if (STREAM) __builtin_nontemporal_store(x, static_cast<V *>(p));

@@ -389,6 +389,22 @@ def test_cache_write_of_long_prompts(dev, tokens, heads, dim, kind):
         assert_cache_holds(cache, want)
 
 
+@pytest.mark.parametrize("kind, out_dtype", [(E4M3, BF16), (BF16, F32), (BF16, BF16)])
+def test_cache_read_of_long_prompts(dev, kind, out_dtype):
+    """Outputs of up to 32 MiB and larger ones, which are stored past the caches, are the cache's values alike."""
+    heads, dim, page = 8, 128, 64
+    most = (32 << 20) // (2 * heads * dim * out_dtype.itemsize)
+    cache = filled_cache(dev, 40, heads, page, dim, kind)
+    values = [t.to(out_dtype) for t in cache_values(cache)]
+    slots = torch.randint(-1, 40 * page, (most + 1,), generator=gen(4)).to(torch.int32)
+    live = (slots >= 0)[:, None, None]
+    at = slots.clamp(min=0).long()
+    for tokens in (most, most + 1):
+        got = ops().kv_cache_read(cache, slots[:tokens].to(dev), out_dtype=out_dtype)
+        for g, v in zip(got, values):
+            assert torch.equal(g.cpu(), torch.where(live, v[at // page, :, at % page], 0)[:tokens])
+
+
 def test_cache_layouts(dev):
     """Parts of a fused projection, [B,H,S,D] memory, unaligned rows, [B,S] slots."""
     b, s, heads, dim = 3, 5, 2, 64

@@ -911,6 +911,27 @@ def test_drafts_agree_with_attention_over_whole_sequences(dev):
     assert torch.equal(o.fmha(bhsd[0], *outs, scale=D ** -0.5, causal=True, out_dtype=F32).transpose(1, 2), whole)
 
 
+def test_a_prompt_continues_a_cached_prefix(dev):
+    """More new tokens than one call takes, grouped heads: written and attended to in chains of up to 64."""
+    o = ops()
+    B, H, Hk, D, page, new = 2, 8, 2, 64, 16, 150
+    prefix, width = [70, 33], 14
+    cache = filled_cache(dev, 30, Hk, page, D, BF16)
+    table = make_table(B, width, 30, 4)
+    q, k, v = (normal(i, B, new, h, D, dtype=BF16).to(dev) for i, h in ((1, H), (2, Hk), (3, Hk)))
+    key = torch.tensor(prefix)[:, None] + torch.arange(new)
+    slots = (table.gather(1, key // page) * page + key % page).to(torch.int32).to(dev)
+    parts = []
+    for at in range(0, new, 64):
+        now = slice(at, at + 64)
+        o.kv_cache_write(cache, k[:, now], v[:, now], slots[:, now].contiguous())
+        context = torch.tensor([p + at for p in prefix], dtype=torch.int32, device=dev)
+        parts.append(o.fmha_cache(q[:, now], cache, table.to(dev), context, scale=D ** -0.5, out_dtype=F32))
+    want, arith, weight = ref.fmha_cache(q.cpu(), *cache_values(cache), table, prefix, None, None, D ** -0.5,
+                                         torch.zeros(q.shape))
+    within(torch.cat(parts, 1), want, arith + 2.0 ** -24 * 2 * weight)
+
+
 def test_captured_steps_replay(dev):
     """Two captured steps and the backward pass, replayed with eager work between and with inputs that change."""
     o = ops()

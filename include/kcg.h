@@ -259,8 +259,10 @@ KCG_API int kcg_softmax_f32(float *x, int64_t rows, int64_t n, void *stream);
 /* Everything in this section is an extension: the reference has no normalisation, no position
  * rotation and no cache.  The entry points form one chain: kcg_qk_norm_rope makes the queries
  * and keys that kcg_fmha_* and the cache take, kcg_kv_cache_write puts new keys and values into
- * the cache, kcg_fmha_cache attends over it, kcg_kv_cache_read brings cached tokens back as
- * rows (a prefill that continues a cached prefix runs kcg_fmha_* on them).
+ * the cache, kcg_fmha_cache attends over it (a prompt that continues a cached prefix goes through it 64
+ * tokens at a time), kcg_kv_cache_read brings cached tokens back as rows.  kcg_fmha_* runs on such rows where
+ * there are as many key heads as query heads, and over all tokens of a sequence: it has no form for fewer
+ * queries than keys.
  *
  * kcg_rows: a tensor [B][S][H][D] whose rows of D elements are contiguous.  Strides are in
  * elements, 0 or more; a tensor that is written has rows that do not overlap (else

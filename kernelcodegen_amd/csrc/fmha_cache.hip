@@ -12,7 +12,9 @@
 //    waits only for its own loads (vmcnt).  The next K is under way while weights and output are computed,
 //    the next V while the scores are; the other workgroups of the CU cover the rest.  (A ring of two of each
 //    took twice the LDS and the same time, and with bf16 pages of 128 left one workgroup to a CU: 96 us
-//    against 72 for 8 x 16 drafts over 8192 keys.)
+//    against 72 for 8 x 16 drafts over 8192 keys.)  One variant has no registers left for the lanes' load offsets
+//    and keeps them in scratch memory: with fp32 output, bf16 pages of 128 and two tiles a reload sits between
+//    the requests of a chunk's K, each of which then waits for the one before.
 //  * S^T = K . Q^T (v_mfma_f32_32x32x16_bf16): the A operand is K rows as ds_read_b128, e4m3 bytes
 //    becoming bf16 with the row's power of two in the conversion itself; B is Q, in registers.  A lane
 //    then holds one query and 16 of the 32 keys, which is the B operand of O^T += V^T . P^T as it
@@ -31,10 +33,11 @@
 //    sequences a launch of one workgroup does that first.  A sequence that fits one unit is written at
 //    once; the others leave normalised partial outputs and the logarithms of their sums in the
 //    workspace, joined by a last launch.
-// Measured: 64 single tokens over contexts to 8192, 32 query heads on 8 of 128, e4m3: 106 us (542 MB, 5.1 TB/s: HBM);
-// one token over 2048 keys: 7.6 us and 3.9 for joining, each a chain of dependent loads; a tree of 32
-// over 131072 keys: 100 us and 8 for joining (69 GFLOP, 0.69 PFLOP/s).  The last is bound by the vector
-// units, busy 52 % of the time (conversions of e4m3, exponentials), beside 35 % of matrix time.
+// Measured: 64 single tokens over contexts to 8192, 32 query heads on 8 of 128, e4m3: 105 to 111 us by the lengths
+// (542 MB, 4.9 to 5.15 TB/s: HBM); one token over 2048 keys: 8.0 us and 4.8 for joining, each a chain of dependent
+// loads; a tree of 32 over 131072 keys: 106 to 111 us with the joining (9), 69 GFLOP, 0.65 PFLOP/s.  In the last
+// neither unit is full: the vector units are busy 52 % of the time (conversions of e4m3, exponentials), the matrix
+// units 35 %, both at once 13 %, and about a quarter of the time neither is.
 #include "kv_cache.h"
 
 namespace kcg {
@@ -821,13 +824,17 @@ inline FcPlan plan_fmha_cache(const kcg_kv_cache &c, int width, int B, int N, in
   const int64_t per_unit = static_cast<int64_t>(c.heads) * p.tiles;
   const int64_t round = 2 * kNumCu / per_unit;  // units that run at once, two workgroups to a CU
   // A few sequences: one round, less the unit that each one's remainder may add (a tree of 32 over 131072
-  // keys: 119 us, with two rounds 130, with four 168).  Many: one and a half, since lengths differ (64
-  // single tokens over contexts to 8192: 121 us, with one round 126; where they do not, 24 over 4000: 45 us,
-  // whole 44; 16: 35 and 42).
+  // keys: 111 us, with two rounds 121, with four 142; 8 single tokens over 4000: 22, 25 and 29, whole 40).  Many:
+  // one and a half (64 single tokens over contexts to 8192: 111 us, with one round 113, with two 106; 24 over 4000:
+  // 45, 51 and 50).  That pays where lengths differ or the chip is not full (32 query heads on 8 of 128, e4m3, cut
+  // and whole): 64 to 8192 111 and 115, 32 64 and 79, 16 39 and 73, 12 x 8 drafts to 20000 62 and 169.  It costs
+  // where whole sequences fill the chip evenly, or where the third launch weighs: 64 over 4096 97 and 92, 32 x 4
+  // drafts over 4000 54 and 49, 24 over 1000 and 16 x 4 over 1000 19 and 16, 128 over 2000 95 and 88, 128 to 2000 65
+  // and 56.  A call with a workspace of no bytes cuts nothing.
   p.few = 8 * static_cast<int64_t>(B) <= round;
   int64_t want = p.few ? round - B : 3 * round / 2;
   const int64_t chunks = (static_cast<int64_t>(width) * c.page_size + kFcChunk - 1) / kFcChunk;
-  // (1 x 4 heads over 500 keys: 9.5 us whole, 10.4 in four units, and two launches more to ask for; 750: 11.4, 10.1)
+  // (1 x 4 drafts over 500 keys, e4m3: 10.1 us whole, 11.0 cut; 750: 12.3 and 11.6; 24 single tokens over 1000: 15.6, 18.6)
   if (chunks <= kFcWhole) return p;
   for (; want > 0; want /= 2) {  // (less, where the workspace does not hold what is preferred)
     const int64_t slots = B < want ? want + B : 2 * want;  // see FcUnit
@@ -896,7 +903,7 @@ int fmha_cache(const kcg_rows &q, const kcg_kv_cache &cache, const int32_t *tabl
   a.q_flip = scale < 0.0f ? 0x80008000u : 0u;
   a.c = scale == 0.0f ? 1.17549435e-38f : fabsf(scale) * 1.44269504088896340736f;
   // Past the caches where the table has room for more than most of the last-level cache (256 MiB): 64 single
-  // tokens over contexts to 8192 (1 GiB of room) 111 us so, 121 otherwise, 8 over 4000 (64 MiB) 22.0 and 20.9.
+  // tokens over contexts to 8192 (1 GiB of room) 111 us so, 122 otherwise, 8 over 4000 (64 MiB) 22.6 and 22.0.
   a.stream = static_cast<int64_t>(B) * width * cache.page_size * cache.heads * cache.dim * 2 * static_cast<int64_t>(sizeof(C)) >
              (int64_t{192} << 20);
   a.vec = rows_aligned16(q, KCG_BF16, B, N, Hq) && rows_aligned16(out, o_dtype, B, N, Hq);

@@ -11,7 +11,9 @@
 // 10^6 times a frequency near 1 has only four bits behind the point in fp32.
 // Measured on bf16 heads of 128: 16384 tokens of 64 heads 98 us (537 MB, 5.5 TB/s), the gradient for
 // 8192 tokens of 40 heads 43 us (252 MB, 5.8 TB/s) and 5 us more for the sum of the weights' shares;
-// 8 tokens 3.2 us.  Requesting a row ahead of its turn made the gradient a quarter slower.
+// 8 tokens 3.2 us.  fp32: 4096 tokens of 64 heads 63 us (268 MB, 4.3 TB/s), 8192 124 us, the gradient for 4096
+// tokens of 40 heads 53 us with the sum (252 MB).  Requesting a row ahead of its turn made the gradient a
+// quarter slower.
 #include "rows.h"
 
 namespace kcg {
@@ -280,7 +282,9 @@ int run_norm_rope(const NormRopeArgs<T> &a, T *gq, T *gk, hipStream_t stream) {
   if (!a.partial) {
     const unsigned grid = static_cast<unsigned>((items + kNrWaves - 1) / kNrWaves);
     // Outputs of the last-level cache's size (256 MiB) and more go past it: 16384 tokens of 64 heads of 128 in
-    // bf16 take 100 us so, 106 otherwise; half as many 55 and 48.
+    // bf16 take 99 us so, 106 otherwise.  Smaller ones are left to their reader: 8192 tokens take 52 us past the
+    // caches and 57 through them, 4096 24 and 31, but with a pass over the outputs behind 95 either way, and 52 past
+    // them and 50 through them (16384: 193 and 187).
     if (VEC && static_cast<int64_t>(a.tokens) * a.rows * D * static_cast<int64_t>(sizeof(T)) >= int64_t{256} << 20)
       return launch(qk_norm_rope_kernel<T, D, VEC, INTERLEAVED, VEC>, dim3(grid), dim3(64 * kNrWaves), 0, stream, a);
     return launch(qk_norm_rope_kernel<T, D, VEC, INTERLEAVED, false>, dim3(grid), dim3(64 * kNrWaves), 0, stream, a);

@@ -282,7 +282,9 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, interl
     last axis, so parts of a fused projection's output are taken as they are.  positions: int32
     [B,S]; inv_freq: fp32, one frequency per rotated pair (2 * len(inv_freq) elements of a head
     are rotated: elements i and i + len, or 2i and 2i + 1 if `interleaved`).  Returns the new
-    (q, k), written to the pair `out` if given; out=(q, k) works in place.  kcg_qk_norm_rope.
+    (q, k), written to the pair `out` if given; out=(q, k) works in place.  Like every operator here it
+    records nothing for autograd, also where an input requires a gradient: qk_norm_rope_backward is called
+    by hand.  kcg_qk_norm_rope.
     """
     index, rq, rk, args = _norm_rope_args(q, k, q_weight, k_weight, positions, inv_freq, eps, interleaved)
     if out is None:

@@ -178,15 +178,15 @@ __global__ __launch_bounds__(256) void kv_cache_read_kernel(const KvMoveArgs<T, 
 template <typename T, typename C, int D, bool VEC>
 int run_write(const KvMoveArgs<const T, C> &a, hipStream_t stream) {
   // Launches of 8192 tokens at most: the comparison grows with their square (131072 tokens, 8 heads of 128:
-  // 617 us in one launch, 300 so; 16384: 35 to 38), and a later launch writes after an earlier one, as
+  // 616 us in one launch, 314 so; 16384: 38 either way), and a later launch writes after an earlier one, as
   // its tokens have to.
   KvMoveArgs<const T, C> part = a;
   for (part.first = 0; part.first < a.tokens; part.first = part.end) {
     part.end = a.tokens - part.first > 8192 ? part.first + 8192 : a.tokens;
     const int n = part.end - part.first;
-    // One token to a workgroup where that fills the chip less than once (64 tokens: 3.5 us, with four 4.9);
-    // more where there are more workgroups than places (4096: 9.0 with two, 9.8 with four, 11.6 with one;
-    // 8191: 14.7 with four, 16.1 with two, 20.8 with one).
+    // One token to a workgroup where that fills the chip less than once (64 tokens: 3.4 us, with four 5.3);
+    // more where there are more workgroups than places (4096: 9.3 with two, 10.9 with four, 10.6 with one;
+    // 8191: 15.2 with four, 16.3 with two, 19.8 with one).
     const int e = n < 2048 ? launch(kv_cache_write_kernel<T, C, D, VEC, 1>, dim3(n), dim3(256), 0, stream, part)
                   : n < 6144 ? launch(kv_cache_write_kernel<T, C, D, VEC, 2>, dim3((n + 1) / 2), dim3(256), 0, stream, part)
                              : launch(kv_cache_write_kernel<T, C, D, VEC, 4>, dim3((n + 3) / 4), dim3(256), 0, stream, part);
